@@ -513,6 +513,178 @@ int llmq_tp_wait_timeout_check(int which, unsigned polls, int *err_word, float *
 int qmatmul_device_noalloc(const float *A, int M, int K, const signed char *Wq, const float *Wscale, int N,
                            float *C, void *stream);
 
+/* ========================================================================= */
+/* Serving operators on device memory (no counterpart in the reference)       */
+/* ========================================================================= */
+/* What a server of many sequences needs next to the decode step: keys and
+ * values in pages, tables of them built on the GPU, the pages' writer,
+ * attention of one new token a row over them, and one sampler call for a batch
+ * of logits rows.
+ *
+ * Each call takes descriptors of buffers the caller holds on the current GPU
+ * and only enqueues work on `stream` (a cudaStream_t; NULL: the default
+ * stream).  Nothing is allocated or kept: a call may be captured into a CUDA
+ * graph, and calls on different streams may overlap unless they share an output
+ * or a workspace.  Pointers marked "or NULL" are optional.  Sizes, strides and
+ * null pointers are checked on the host, and so is that every buffer is memory
+ * of the current GPU; a call that fails one of these checks returns
+ * LLMQ_ERR_ARG and enqueues nothing.  Values that only the GPU sees (lengths,
+ * page ids, slots, positions) are checked there: an entry out of range is left
+ * out and its flag is OR'ed into *status (a device int the caller has zeroed, or
+ * NULL).  Unused descriptor fields must be zero.  Strides count elements.
+ * Returns 0 or an error code. */
+
+/* element types */
+enum { LLMQ_F32 = 0, LLMQ_F16 = 1, LLMQ_BF16 = 2 };
+
+/* flags of a status word */
+enum {
+  LLMQ_PAGED_BAD_LEN = 1,   /* a length below 0 or past the table's row */
+  LLMQ_PAGED_NO_PAGES = 2,  /* free pages ran out */
+  LLMQ_PAGED_NO_ROWS = 4,   /* more rows than max_rows */
+  LLMQ_PAGED_BAD_PAGE = 8,  /* a page id outside the pool, or missing */
+  LLMQ_PAGED_BAD_SLOT = 16, /* a slot past the pool */
+  LLMQ_PAGED_BAD_POS = 32   /* a position outside the angle tables */
+};
+
+/* A pool of pages of keys and values.  Element (page, token, head, d) of k is
+ * k[page * page_stride + token * token_stride + head * head_stride + d], the
+ * same for v, so [page][token][head][d] and [page][head][token][d] pools are
+ * both described.  k and v start on 16 bytes and the strides are multiples of
+ * 16 bytes.  Slot s is token s % page_size of page s / page_size. */
+typedef struct {
+  void *k, *v;
+  int dtype;
+  int n_pages, page_size; /* n_pages * page_size < 2^31 */
+  int n_kv, head_dim;     /* head_dim: a multiple of 8, at most 256 */
+  int reserved;
+  long long page_stride, token_stride, head_stride;
+} LlmqPagedKV;
+
+/* Block tables and slot maps of one step, from the requests' lengths.
+ * Request b has cached[b] tokens in its pages (table row b, the first
+ * ceil(cached[b] / page_size) entries) and brings added[b] more.  The pages it
+ * lacks are taken from free_pages in the order of the requests, starting at
+ * free_pages[*free_head], and written into its row.  The step's rows are the
+ * added tokens of request 0, then of request 1, and so on.
+ *   lens[b]   cached + added                first[b]  first row of request b; first[n_seqs]: rows in all
+ *   slots[r]  the row's slot (-1: padding)  positions[r]  its position in the sequence (-1)
+ *   seqs[r]   its request (-1)              spans[r]  positions[r] + 1: what the row may attend (0)
+ * Rows from first[n_seqs] to max_rows are padding.  *next_head receives the
+ * position after the last page taken; it may be free_head itself, and lens may
+ * be cached.  A request that cannot be served adds nothing (its lens stay
+ * cached): one whose lengths are below 0 or pass the row's max_pages, whose
+ * rows (counted over the requests of valid lengths before it) pass max_rows, or
+ * whose pages (counted over the requests with rows before it) pass n_free; a
+ * request that needs no page is not held up by the last.  A request whose
+ * cached length is itself out of range gets lens 0. */
+typedef struct {
+  int n_seqs, page_size, max_pages, max_rows, n_free;
+  int reserved;
+  const int *cached, *added;  /* [n_seqs] */
+  const int *free_pages;      /* [n_free] */
+  const int *free_head;       /* or NULL: 0 */
+  int *table;                 /* [n_seqs][table_stride] */
+  long long table_stride;
+  int *lens, *first;          /* [n_seqs], [n_seqs + 1] */
+  long long *slots;           /* [max_rows] */
+  int *positions, *seqs, *spans; /* [max_rows], each or NULL */
+  int *next_head;             /* or NULL */
+  int *status;                /* or NULL */
+} LlmqPagedPlan;
+int llmq_paged_plan(const LlmqPagedPlan *a, void *stream);
+
+/* Writes a step's keys and values into their slots, and rotates q and k
+ * (rope.c:48-68: pairs (d, d + head_dim / 2), in f32) when angle tables are
+ * given.  Row r of k and v holds n_kv heads of head_dim, of q n_heads; rows are
+ * *_stride apart, so the three may be parts of one packed row.  q_out may be q.
+ * Values are rounded once, to the pool's type (q_out: to dtype).  A row whose
+ * slot is below 0 is left out (q_out keeps what it held).  Two rows with one
+ * slot leave either's values there. */
+typedef struct {
+  int n_rows, n_heads; /* n_heads: 0 without q */
+  int dtype;           /* of q, k, v and q_out */
+  int rope_len;        /* positions in the angle tables */
+  const void *q, *k, *v;
+  long long q_stride, k_stride, v_stride;
+  void *q_out;
+  long long q_out_stride;
+  const long long *slots;  /* [n_rows] */
+  const int *positions;    /* [n_rows]; or NULL without tables */
+  const float *rope_cos, *rope_sin; /* [rope_len][head_dim / 2], or both NULL */
+  int *status;             /* or NULL */
+} LlmqPagedAppend;
+int llmq_paged_append(const LlmqPagedKV *kv, const LlmqPagedAppend *a, void *stream);
+
+/* Attention of one query row a sequence over a paged cache: row r attends
+ * positions [max(0, n - window), n), n = lens[r] (window 0: from 0), of the
+ * sequence in table row seqs[r] (NULL: row r):
+ *   out = sum_p exp(s_p - m) v_p / sum_p exp(s_p - m),  s_p = scale * <q, k_p>
+ * and lse[r][h] = m + log sum_p exp(s_p - m).  n_heads / n_kv query heads share
+ * a KV head.  q is in dtype; the pool has the same type, or any type when dtype
+ * is LLMQ_F32.  Scores, maxima, sums and the output are formed in f32 and
+ * rounded once; with a 16-bit dtype the weights are rounded to it before they
+ * multiply the values.  A row without positions gives zeros and lse -infinity.
+ * Positions on a page outside the pool are left out.  What the pool holds past
+ * a row's length is never read into a result.  scale 0 stands for
+ * 1 / sqrt(head_dim).  The workspace need not be initialised; calls that may
+ * overlap need one each. */
+typedef struct {
+  int n_rows, n_heads;
+  int dtype;     /* of q and out */
+  int window;
+  int max_pages; /* entries of a table row */
+  int n_seqs;    /* table rows */
+  float scale;
+  int reserved;
+  const void *q;          /* [n_rows][n_heads][head_dim], rows q_stride apart */
+  long long q_stride;
+  void *out;              /* as q; rows out_stride apart */
+  long long out_stride;
+  float *lse;             /* [n_rows][n_heads], or NULL */
+  const int *table;       /* [n_seqs][table_stride] page ids */
+  long long table_stride;
+  const int *seqs;        /* [n_rows], or NULL */
+  const int *lens;        /* [n_rows] */
+  void *workspace;        /* 16-byte aligned; llmq_paged_attention_workspace bytes */
+  size_t workspace_bytes;
+  int *status;            /* or NULL */
+} LlmqPagedAttention;
+int llmq_paged_attention(const LlmqPagedKV *kv, const LlmqPagedAttention *a, void *stream);
+/* Bytes of workspace such a call needs on any sm_100 GPU (0 on bad sizes, with
+ * the error set). */
+size_t llmq_paged_attention_workspace(int n_rows, int n_heads, int n_kv, int head_dim);
+
+/* Draws one token a row from given random numbers, by the rules of sample_token
+ * (sampler.c:60-115) with min-p added.  With w_j = exp((l_j - max l) / T) and
+ * the tokens in order of falling logit (the lower index first among equal
+ * ones), kept is the shortest of: the first top_k (off: <= 0 or >= vocab); those
+ * with w >= min_p (off: <= 0; above 1 counts as 1); and the first tokens whose
+ * sum of w reaches top_p of the whole row's (off: outside (0, 1)).  The token
+ * drawn is the first one, in that order, at which the sum of w reaches u times
+ * the kept sum; u is clamped to [0, 1] (NaN: 0).  A temperature that is not above
+ * 0 (NaN too) takes the first largest logit.  Sums are exact to 2^-42 of the
+ * largest w or better (64-bit integers, the same in any order), so a row's
+ * token does not depend on the batch it is in.  A NaN or -infinite logit is
+ * never drawn; a row of nothing else gives id -1 and logprob -infinity; among
+ * +infinite logits the weights are equal.
+ * logprobs[r] is the log of the drawn token's share of the kept sum (0 for the
+ * greedy choice). */
+typedef struct {
+  int n_rows, vocab; /* vocab: at most 2^20 */
+  int dtype;
+  int reserved;
+  const void *logits;        /* [n_rows][vocab], rows `stride` apart */
+  long long stride;
+  const float *temperature;  /* [n_rows], or NULL: 1 */
+  const int *top_k;          /* [n_rows], or NULL: off */
+  const float *top_p, *min_p; /* [n_rows], each or NULL: off */
+  const float *u;            /* [n_rows] random numbers in [0, 1) */
+  int *ids;                  /* [n_rows] */
+  float *logprobs;           /* [n_rows], or NULL */
+} LlmqSampleRows;
+int llmq_sample_rows(const LlmqSampleRows *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,501 @@
+// llmq_paged.cu - the paged key-value cache on device memory: block tables and
+// slot maps from request lengths (llmq_paged_plan), the cache's writer with
+// RoPE (llmq_paged_append), and attention of one query row a sequence
+// (llmq_paged_attention).
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "llmq_serve.cuh"
+
+using namespace llmq;
+
+namespace {
+
+// ==================================================================== plan
+constexpr int kScanThreads = 1024;
+
+// Inclusive sum over the block's threads; *total receives the block's sum.
+__device__ __forceinline__ long long block_scan(long long v, long long *warp_sums, long long *total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  long long w = warp_sums[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += u;
+  }
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return v + (warp ? before : 0);
+}
+
+// One CTA: requests in chunks of 1024, one a thread.  Three sums in order:
+// rows over the requests of valid lengths (which of them fit max_rows), pages
+// over those (which fit the free pages), rows over what is served.  The chunk's
+// new pages are then written by all threads, each finding its request by
+// bisection of the page sums.
+__global__ void __launch_bounds__(kScanThreads) k_plan_scan(const LlmqPagedPlan a) {
+  __shared__ long long s_warp[32];
+  __shared__ long long s_end[kScanThreads];  // page sums up to and with each request
+  __shared__ int s_have[kScanThreads], s_new[kScanThreads];
+  serve_wait();
+  serve_dependents();
+  const int tid = threadIdx.x;
+  const long long head = a.free_head ? max(*a.free_head, 0) : 0;
+  const long long cap = (long long)a.max_pages * a.page_size;
+  long long rows_seen = 0, pages_seen = 0, rows_done = 0, pages_done = 0;
+  int flags = a.free_head && *a.free_head < 0 ? LLMQ_PAGED_NO_PAGES : 0;
+  const bool bad_head = flags != 0;
+  for (int b0 = 0; b0 < a.n_seqs; b0 += kScanThreads) {
+    const int b = b0 + tid;
+    const bool in = b < a.n_seqs;
+    const long long cached = in ? a.cached[b] : 0, added = in ? a.added[b] : 0;
+    const bool held = cached >= 0 && cached <= cap;
+    const bool valid = held && added >= 0 && cached + added <= cap;
+    if (in && !valid) flags |= LLMQ_PAGED_BAD_LEN;
+    long long total;
+    const long long want = valid ? added : 0;
+    const long long rows = rows_seen + block_scan(want, s_warp, &total);
+    rows_seen += total;
+    const bool fits = valid && (want == 0 || rows <= a.max_rows);
+    if (valid && !fits) flags |= LLMQ_PAGED_NO_ROWS;
+    const long long have = (cached + a.page_size - 1) / a.page_size;
+    const long long need = fits ? (cached + added + a.page_size - 1) / a.page_size - have : 0;
+    const long long pages = pages_seen + block_scan(need, s_warp, &total);
+    pages_seen += total;
+    const bool served = fits && (need == 0 || (!bad_head && head + pages <= a.n_free));
+    if (fits && !served) flags |= LLMQ_PAGED_NO_PAGES;
+    const long long mine = served ? added : 0;
+    const long long end = rows_done + block_scan(mine, s_warp, &total);
+    rows_done += total;
+    if (in) {
+      a.first[b] = static_cast<int>(end - mine);
+      a.lens[b] = held ? static_cast<int>(cached + mine) : 0;
+    }
+    // pages taken: a prefix of the requests that need any, so `pages` is their sum too
+    const int fresh = served ? static_cast<int>(need) : 0;
+    const long long taken = pages_done + block_scan(fresh, s_warp, &total);
+    s_end[tid] = taken;
+    s_have[tid] = static_cast<int>(have);
+    s_new[tid] = fresh;
+    __syncthreads();
+    for (long long j = pages_done + tid; j < pages_done + total; j += kScanThreads) {
+      int lo = 0, hi = kScanThreads - 1;  // the first request whose sum passes j
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_end[mid] > j)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      const int at = s_have[lo] + static_cast<int>(j - (s_end[lo] - s_new[lo]));
+      a.table[(long long)(b0 + lo) * a.table_stride + at] = a.free_pages[head + j];
+    }
+    pages_done += total;
+    __syncthreads();
+  }
+  if (tid == 0) {
+    a.first[a.n_seqs] = static_cast<int>(rows_done);
+    if (a.next_head) *a.next_head = bad_head ? *a.free_head : static_cast<int>(head + pages_done);
+  }
+  if (flags && a.status) atomicOr(a.status, flags);
+}
+
+constexpr int kFillThreads = 256;
+
+__global__ void __launch_bounds__(kFillThreads) k_plan_fill(const LlmqPagedPlan a) {
+  serve_wait();
+  serve_dependents();
+  const int r = blockIdx.x * kFillThreads + threadIdx.x;
+  if (r >= a.max_rows) return;
+  int seq = -1, pos = -1;
+  long long slot = -1;
+  if (r < a.first[a.n_seqs]) {
+    int lo = 0, hi = a.n_seqs - 1;  // the last request that starts at or before r
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.first[mid] <= r)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    seq = lo;
+    pos = a.lens[seq] - (a.first[seq + 1] - r);
+    const int page = a.table[(long long)seq * a.table_stride + pos / a.page_size];
+    if (page >= 0)
+      slot = (long long)page * a.page_size + pos % a.page_size;
+    else if (a.status)
+      atomicOr(a.status, LLMQ_PAGED_BAD_PAGE);
+  }
+  a.slots[r] = slot;
+  if (a.positions) a.positions[r] = pos;
+  if (a.seqs) a.seqs[r] = seq;
+  if (a.spans) a.spans[r] = pos + 1;
+}
+
+// ================================================================== append
+struct AppendArgs {
+  LlmqPagedKV kv;
+  LlmqPagedAppend a;
+};
+
+constexpr int kAppendThreads = 256;
+constexpr int kHeadLanes = 8;
+
+// A thread owns VN adjacent pairs (d, d + head_dim / 2) of every eighth head of
+// a row: the pairs' angles are read once and serve its heads.
+template <typename T, typename KT, int VN>
+__global__ void __launch_bounds__(kAppendThreads) k_append(const AppendArgs p, int chunks, int lanes) {
+  serve_wait();
+  serve_dependents();
+  const LlmqPagedKV &kv = p.kv;
+  const LlmqPagedAppend &a = p.a;
+  const int per_row = chunks * lanes, rows_here = kAppendThreads / per_row;
+  const int sub = threadIdx.x / per_row, t = threadIdx.x - sub * per_row;
+  const int r = blockIdx.x * rows_here + sub;
+  if (sub >= rows_here || r >= a.n_rows) return;
+  const int hl = t / chunks, half = kv.head_dim / 2, d = (t - hl * chunks) * VN;
+  const long long slot = a.slots[r];
+  if (slot < 0) return;
+  if (slot >= (long long)kv.n_pages * kv.page_size) {
+    if (t == 0 && a.status) atomicOr(a.status, LLMQ_PAGED_BAD_SLOT);
+    return;
+  }
+  const bool turn = a.rope_cos != nullptr;
+  Pack<float, VN> cs, sn;
+  if (turn) {
+    const int pos = a.positions[r];
+    if (pos < 0 || pos >= a.rope_len) {
+      if (t == 0 && a.status) atomicOr(a.status, LLMQ_PAGED_BAD_POS);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      cs.v[i] = a.rope_cos[(size_t)pos * half + d + i];
+      sn.v[i] = a.rope_sin[(size_t)pos * half + d + i];
+    }
+  }
+  const long long page = slot / kv.page_size, token = slot % kv.page_size;
+  const long long at = page * kv.page_stride + token * kv.token_stride;
+  const int nq = a.q ? a.n_heads : 0;
+  for (int h = hl; h < nq + 2 * kv.n_kv; h += lanes) {
+    const bool is_q = h < nq, is_k = !is_q && h < nq + kv.n_kv;
+    const int hh = is_q ? h : is_k ? h - nq : h - nq - kv.n_kv;
+    const T *src = is_q   ? static_cast<const T *>(a.q) + r * a.q_stride
+                   : is_k ? static_cast<const T *>(a.k) + r * a.k_stride
+                          : static_cast<const T *>(a.v) + r * a.v_stride;
+    src += (size_t)hh * kv.head_dim + d;
+    const Pack<T, VN> x = *reinterpret_cast<const Pack<T, VN> *>(src);
+    const Pack<T, VN> y = *reinterpret_cast<const Pack<T, VN> *>(src + half);
+    Pack<float, VN> u, w;
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      u.v[i] = to_f32(x.v[i]);
+      w.v[i] = to_f32(y.v[i]);
+      if (turn && (is_q || is_k)) {  // rope.c:58-64, the products rounded on their own
+        const float a0 = u.v[i], b0 = w.v[i];
+        u.v[i] = __fsub_rn(__fmul_rn(a0, cs.v[i]), __fmul_rn(b0, sn.v[i]));
+        w.v[i] = __fadd_rn(__fmul_rn(b0, cs.v[i]), __fmul_rn(a0, sn.v[i]));
+      }
+    }
+    auto put = [&](auto *dst) {
+      using D = std::remove_pointer_t<decltype(dst)>;
+      Pack<D, VN> lo, hi;
+#pragma unroll
+      for (int i = 0; i < VN; ++i) {
+        lo.v[i] = from_f32<D>(u.v[i]);
+        hi.v[i] = from_f32<D>(w.v[i]);
+      }
+      *reinterpret_cast<Pack<D, VN> *>(dst) = lo;
+      *reinterpret_cast<Pack<D, VN> *>(dst + half) = hi;
+    };
+    if (is_q)
+      put(static_cast<T *>(a.q_out) + r * a.q_out_stride + (size_t)hh * kv.head_dim + d);
+    else
+      put(static_cast<KT *>(is_k ? kv.k : kv.v) + at + hh * kv.head_stride + d);
+  }
+}
+
+// =============================================================== attention
+struct AttendArgs {
+  LlmqPagedKV kv;
+  LlmqPagedAttention a;
+};
+
+constexpr int kAttendWarps = 4;
+
+// One CTA a (row, KV head, query head of its group): the warps share out the
+// positions, a lane owns the dims lane, lane + 32, ...; each warp keeps its own
+// running maximum and sum, joined at the end in shared memory.
+template <typename T, typename KT>
+__global__ void __launch_bounds__(kAttendWarps * 32) k_attend_plain(const AttendArgs p) {
+  constexpr int kPer = 8;  // dims a lane, head_dim <= 256
+  __shared__ float s_o[kAttendWarps][256];
+  __shared__ float s_m[kAttendWarps], s_l[kAttendWarps];
+  serve_wait();
+  serve_dependents();
+  const LlmqPagedKV &kv = p.kv;
+  const LlmqPagedAttention &a = p.a;
+  const int r = blockIdx.y, h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = kv.head_dim;
+  const int kvh = h / (a.n_heads / kv.n_kv);
+  const int seq = a.seqs ? a.seqs[r] : r;
+  long long n = a.lens[r];
+  const long long cap = (long long)a.max_pages * kv.page_size;
+  int flags = 0;
+  if (n < 0 || n > cap || ((seq < 0 || seq >= a.n_seqs) && n > 0)) {
+    flags |= LLMQ_PAGED_BAD_LEN;
+    n = seq < 0 || seq >= a.n_seqs || n < 0 ? 0 : cap;
+  }
+  const long long n0 = a.window > 0 && n > a.window ? n - a.window : 0;
+  const T *q = static_cast<const T *>(a.q) + r * a.q_stride + (size_t)h * hd;
+  float qv[kPer], o[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int d = lane + 32 * i;
+    qv[i] = d < hd ? to_f32(q[d]) : 0.0f;
+    o[i] = 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f;
+  for (long long pos = n0 + warp; pos < n; pos += kAttendWarps) {
+    const int page = a.table[seq * a.table_stride + pos / kv.page_size];
+    if (page < 0 || page >= kv.n_pages) {
+      flags |= LLMQ_PAGED_BAD_PAGE;
+      continue;
+    }
+    const long long at = page * kv.page_stride + (pos % kv.page_size) * kv.token_stride + kvh * kv.head_stride;
+    const KT *k = static_cast<const KT *>(kv.k) + at, *v = static_cast<const KT *>(kv.v) + at;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int d = lane + 32 * i;
+      if (d < hd) s = fmaf(qv[i], to_f32(k[d]), s);
+    }
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    s *= a.scale;
+    const float mn = fmaxf(m, s);
+    const float c = m == -INFINITY ? 0.0f : expf(m - mn), e = mn == -INFINITY ? 0.0f : expf(s - mn);
+    l = l * c + e;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int d = lane + 32 * i;
+      if (d < hd) o[i] = fmaf(e, to_f32(v[d]), o[i] * c);
+    }
+  }
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (lane + 32 * i < hd) s_o[warp][lane + 32 * i] = o[i];
+  if (flags && lane == 0 && a.status) atomicOr(a.status, flags);
+  __syncthreads();
+  float mx = -INFINITY, sum = 0.0f;
+  for (int w = 0; w < kAttendWarps; ++w) mx = fmaxf(mx, s_m[w]);
+  for (int w = 0; w < kAttendWarps; ++w) sum += mx == -INFINITY ? 0.0f : s_l[w] * expf(s_m[w] - mx);
+  T *out = static_cast<T *>(a.out) + r * a.out_stride + (size_t)h * hd;
+  for (int d = threadIdx.x; d < hd; d += kAttendWarps * 32) {
+    float v = 0.0f;
+    for (int w = 0; w < kAttendWarps; ++w) v += mx == -INFINITY ? 0.0f : s_o[w][d] * expf(s_m[w] - mx);
+    out[d] = from_f32<T>(sum > 0.0f ? v / sum : 0.0f);
+  }
+  if (threadIdx.x == 0 && a.lse) a.lse[(size_t)r * a.n_heads + h] = sum > 0.0f ? mx + logf(sum) : -INFINITY;
+}
+
+// ------------------------------------------------------------- host checks
+void check_pool(ServeCheck &c, const LlmqPagedKV *kv) {
+  c.require(kv != nullptr, "null pool");
+  if (c.rc != LLMQ_OK) return;
+  c.require(kv->k && kv->v, "null pool memory");
+  c.require(serve_dtype(kv->dtype), "unknown type of the pool");
+  c.require(kv->n_pages > 0 && kv->page_size > 0 && (long long)kv->n_pages * kv->page_size <= INT_MAX,
+            "the pool needs n_pages > 0, page_size > 0 and fewer than 2^31 slots");
+  c.require(kv->n_kv > 0 && kv->n_kv <= 65535, "n_kv outside 1..65535");
+  c.require(kv->head_dim > 0 && kv->head_dim <= 256 && kv->head_dim % 8 == 0,
+            "head_dim must be a multiple of 8, at most 256");
+  if (c.rc != LLMQ_OK) return;
+  const long long e = static_cast<long long>(serve_bytes(kv->dtype));
+  c.require(aligned16(kv->k) && aligned16(kv->v), "pool memory must start on 16 bytes");
+  c.require(kv->page_stride >= 0 && kv->token_stride >= 0 && kv->head_stride >= 0 && kv->page_stride * e % 16 == 0 &&
+                kv->token_stride * e % 16 == 0 && kv->head_stride * e % 16 == 0,
+            "pool strides must be multiples of 16 bytes, none negative");
+}
+
+}  // namespace
+
+extern "C" LLMQ_API int llmq_paged_plan(const LlmqPagedPlan *a, void *stream) {
+  ServeCheck c("llmq_paged_plan");
+  c.require(a != nullptr, "null descriptor");
+  if (c.rc != LLMQ_OK) return c.rc;
+  c.require(a->n_seqs >= 0 && a->max_rows >= 0 && a->n_free >= 0, "negative size");
+  c.require(a->page_size > 0 && a->max_pages > 0 && (long long)a->page_size * a->max_pages <= INT_MAX,
+            "page_size and max_pages must be above 0 and their product below 2^31");
+  c.require(a->table_stride >= a->max_pages, "table_stride is below max_pages");
+  c.require(a->n_seqs == 0 || (a->cached && a->added && a->table && a->lens), "null pointer");
+  c.require(a->first && (a->max_rows == 0 || a->slots) && (a->n_free == 0 || a->free_pages), "null pointer");
+  c.on_device();
+  c.memory(a->cached, "cached");
+  c.memory(a->added, "added");
+  c.memory(a->free_pages, "free_pages");
+  c.memory(a->free_head, "free_head");
+  c.memory(a->table, "table");
+  c.memory(a->lens, "lens");
+  c.memory(a->first, "first");
+  c.memory(a->slots, "slots");
+  c.memory(a->positions, "positions");
+  c.memory(a->seqs, "seqs");
+  c.memory(a->spans, "spans");
+  c.memory(a->next_head, "next_head");
+  c.memory(a->status, "status");
+  if (c.rc != LLMQ_OK) return c.rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  c.launched(serve_launch(k_plan_scan, dim3(1), dim3(kScanThreads), 0, st, *a));
+  if (c.rc == LLMQ_OK && a->max_rows > 0)
+    c.launched(serve_launch(k_plan_fill, dim3((a->max_rows - 1) / kFillThreads + 1), dim3(kFillThreads), 0, st, *a));
+  return c.rc;
+}
+
+namespace {
+
+template <typename T, typename KT>
+cudaError_t launch_append(const AppendArgs &p, cudaStream_t st) {
+  const LlmqPagedAppend &a = p.a;
+  constexpr int kWide = 16 / sizeof(T);
+  const int half = p.kv.head_dim / 2;
+  auto wide = [&](const void *x, long long stride) {
+    return !x || (aligned16(x) && stride * (long long)sizeof(T) % 16 == 0);
+  };
+  const bool vec = half % kWide == 0 && wide(a.q, a.q_stride) && wide(a.k, a.k_stride) && wide(a.v, a.v_stride) &&
+                   wide(a.q_out, a.q_out_stride);
+  const int chunks = vec ? half / kWide : half;
+  const int lanes = std::min(kHeadLanes, kAppendThreads / chunks), rows_here = kAppendThreads / (chunks * lanes);
+  const dim3 grid((a.n_rows - 1) / rows_here + 1);
+  return vec ? serve_launch(k_append<T, KT, kWide>, grid, dim3(kAppendThreads), 0, st, p, chunks, lanes)
+             : serve_launch(k_append<T, KT, 1>, grid, dim3(kAppendThreads), 0, st, p, chunks, lanes);
+}
+
+template <typename T, typename KT>
+cudaError_t launch_attend(const AttendArgs &p, cudaStream_t st) {
+  return serve_launch(k_attend_plain<T, KT>, dim3(p.a.n_heads, p.a.n_rows), dim3(kAttendWarps * 32), 0, st, p);
+}
+
+// f(T, KT) for a type of the rows and one of the pool that check_types let through.
+template <typename F>
+cudaError_t by_types(int t, int kt, F f) {
+  if (t == LLMQ_F16) return f(__half(), __half());
+  if (t == LLMQ_BF16) return f(__nv_bfloat16(), __nv_bfloat16());
+  if (kt == LLMQ_F16) return f(float(), __half());
+  if (kt == LLMQ_BF16) return f(float(), __nv_bfloat16());
+  return f(float(), float());
+}
+
+void check_types(ServeCheck &c, int t, int kt) {
+  c.require(serve_dtype(t), "unknown type of the rows");
+  c.require(t == kt || t == LLMQ_F32, "the rows must have the pool's type or be f32");
+}
+
+}  // namespace
+
+extern "C" LLMQ_API int llmq_paged_append(const LlmqPagedKV *kv, const LlmqPagedAppend *a, void *stream) {
+  ServeCheck c("llmq_paged_append");
+  c.require(a != nullptr, "null descriptor");
+  check_pool(c, kv);
+  if (c.rc != LLMQ_OK) return c.rc;
+  check_types(c, a->dtype, kv->dtype);
+  c.require(a->n_rows >= 0 && a->n_heads >= 0 && a->rope_len >= 0, "negative size");
+  if (c.rc != LLMQ_OK || a->n_rows == 0) return c.rc;
+  c.require(a->k && a->v && a->slots, "null pointer");
+  c.require((a->n_heads > 0) == (a->q != nullptr) && (a->q != nullptr) == (a->q_out != nullptr),
+            "q, q_out and n_heads go together");
+  c.require((a->rope_cos != nullptr) == (a->rope_sin != nullptr), "one angle table without the other");
+  c.require(!a->rope_cos || (a->positions && a->rope_len > 0), "angle tables without positions or rope_len");
+  const long long kvd = (long long)kv->n_kv * kv->head_dim, qd = (long long)a->n_heads * kv->head_dim;
+  c.require(a->k_stride >= kvd && a->v_stride >= kvd && a->q_stride >= (a->q ? qd : 0) &&
+                a->q_out_stride >= (a->q ? qd : 0),
+            "a row stride is shorter than its row");
+  const size_t e = c.rc == LLMQ_OK ? serve_bytes(a->dtype) : 1;
+  c.require(aligned_to(a->q, e) && aligned_to(a->k, e) && aligned_to(a->v, e) && aligned_to(a->q_out, e),
+            "a row does not start on an element");
+  c.on_device();
+  c.memory(kv->k, "the pool");
+  c.memory(kv->v, "the pool");
+  c.memory(a->q, "q");
+  c.memory(a->k, "k");
+  c.memory(a->v, "v");
+  c.memory(a->q_out, "q_out");
+  c.memory(a->slots, "slots");
+  c.memory(a->positions, "positions");
+  c.memory(a->rope_cos, "rope_cos");
+  c.memory(a->rope_sin, "rope_sin");
+  c.memory(a->status, "status");
+  if (c.rc != LLMQ_OK) return c.rc;
+  const AppendArgs p{*kv, *a};
+  c.launched(by_types(a->dtype, kv->dtype, [&](auto t, auto kt) {
+    return launch_append<decltype(t), decltype(kt)>(p, static_cast<cudaStream_t>(stream));
+  }));
+  return c.rc;
+}
+
+extern "C" LLMQ_API size_t llmq_paged_attention_workspace(int n_rows, int n_heads, int n_kv, int head_dim) {
+  if (n_rows < 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv != 0 || head_dim <= 0 || head_dim > 256 ||
+      head_dim % 8 != 0) {
+    llmq_set_error(LLMQ_ERR_ARG, "llmq_paged_attention_workspace: bad sizes (%d rows, %d / %d heads of %d)", n_rows,
+                   n_heads, n_kv, head_dim);
+    return 0;
+  }
+  return 16;
+}
+
+extern "C" LLMQ_API int llmq_paged_attention(const LlmqPagedKV *kv, const LlmqPagedAttention *a, void *stream) {
+  ServeCheck c("llmq_paged_attention");
+  c.require(a != nullptr, "null descriptor");
+  check_pool(c, kv);
+  if (c.rc != LLMQ_OK) return c.rc;
+  check_types(c, a->dtype, kv->dtype);
+  c.require(a->n_rows >= 0 && a->n_seqs >= 0 && a->max_pages >= 0 && a->window >= 0, "negative size");
+  c.require(a->n_heads > 0 && a->n_heads % kv->n_kv == 0, "n_heads must be a multiple of n_kv");
+  c.require((long long)a->max_pages * kv->page_size <= INT_MAX, "max_pages * page_size must stay below 2^31");
+  c.require(a->table_stride >= a->max_pages, "table_stride is below max_pages");
+  c.require(std::isfinite(a->scale), "scale is not finite");
+  if (c.rc != LLMQ_OK || a->n_rows == 0) return c.rc;
+  c.require(a->n_rows <= 65535, "more than 65535 rows");
+  c.require(a->q && a->out && a->lens && (a->table || a->max_pages == 0 || a->n_seqs == 0), "null pointer");
+  c.require(a->seqs || a->n_seqs >= a->n_rows, "n_seqs is below n_rows and seqs is null");
+  const long long qd = (long long)a->n_heads * kv->head_dim;
+  c.require(a->q_stride >= qd && a->out_stride >= qd, "a row stride is shorter than its row");
+  const size_t e = c.rc == LLMQ_OK ? serve_bytes(a->dtype) : 1;
+  c.require(aligned_to(a->q, e) && aligned_to(a->out, e), "a row does not start on an element");
+  if (c.rc != LLMQ_OK) return c.rc;
+  const size_t need = llmq_paged_attention_workspace(a->n_rows, a->n_heads, kv->n_kv, kv->head_dim);
+  c.require(a->workspace && a->workspace_bytes >= need && aligned16(a->workspace),
+            "the workspace is missing, too small or not on 16 bytes");
+  c.on_device();
+  c.memory(kv->k, "the pool");
+  c.memory(kv->v, "the pool");
+  c.memory(a->q, "q");
+  c.memory(a->out, "out");
+  c.memory(a->lse, "lse");
+  c.memory(a->table, "table");
+  c.memory(a->seqs, "seqs");
+  c.memory(a->lens, "lens");
+  c.memory(a->workspace, "workspace");
+  c.memory(a->status, "status");
+  if (c.rc != LLMQ_OK) return c.rc;
+  AttendArgs p{*kv, *a};
+  if (p.a.scale == 0.0f) p.a.scale = 1.0f / std::sqrt(static_cast<float>(kv->head_dim));
+  c.launched(by_types(a->dtype, kv->dtype, [&](auto t, auto kt) {
+    return launch_attend<decltype(t), decltype(kt)>(p, static_cast<cudaStream_t>(stream));
+  }));
+  return c.rc;
+}

@@ -69,6 +69,47 @@ class LlmqConfig(C.Structure):
     _fields_ = [(n, C.c_int) for n in CONFIG_FIELDS] + [("rope_base", C.c_float), ("eps", C.c_float)]
 
 
+# Descriptors of the serving operators (llmq_cuda.h): device pointers as
+# integers, strides in elements; fields left out are zero.
+LLMQ_F32, LLMQ_F16, LLMQ_BF16 = range(3)
+(LLMQ_PAGED_BAD_LEN, LLMQ_PAGED_NO_PAGES, LLMQ_PAGED_NO_ROWS, LLMQ_PAGED_BAD_PAGE, LLMQ_PAGED_BAD_SLOT,
+ LLMQ_PAGED_BAD_POS) = (1 << i for i in range(6))
+
+
+def _fields(*groups):
+    return [(n, t) for t, names in groups for n in names.split()]
+
+
+class PagedKV(C.Structure):
+    _fields_ = _fields((C.c_void_p, "k v"), (C.c_int, "dtype n_pages page_size n_kv head_dim reserved"),
+                       (C.c_longlong, "page_stride token_stride head_stride"))
+
+
+class PagedPlan(C.Structure):
+    _fields_ = _fields((C.c_int, "n_seqs page_size max_pages max_rows n_free reserved"),
+                       (C.c_void_p, "cached added free_pages free_head table"), (C.c_longlong, "table_stride"),
+                       (C.c_void_p, "lens first slots positions seqs spans next_head status"))
+
+
+class PagedAppend(C.Structure):
+    _fields_ = _fields((C.c_int, "n_rows n_heads dtype rope_len"), (C.c_void_p, "q k v"),
+                       (C.c_longlong, "q_stride k_stride v_stride"), (C.c_void_p, "q_out"),
+                       (C.c_longlong, "q_out_stride"),
+                       (C.c_void_p, "slots positions rope_cos rope_sin status"))
+
+
+class PagedAttention(C.Structure):
+    _fields_ = _fields((C.c_int, "n_rows n_heads dtype window max_pages n_seqs"), (C.c_float, "scale"),
+                       (C.c_int, "reserved"), (C.c_void_p, "q"), (C.c_longlong, "q_stride"), (C.c_void_p, "out"),
+                       (C.c_longlong, "out_stride"), (C.c_void_p, "lse table"), (C.c_longlong, "table_stride"),
+                       (C.c_void_p, "seqs lens workspace"), (C.c_size_t, "workspace_bytes"), (C.c_void_p, "status"))
+
+
+class SampleRows(C.Structure):
+    _fields_ = _fields((C.c_int, "n_rows vocab dtype reserved"), (C.c_void_p, "logits"), (C.c_longlong, "stride"),
+                       (C.c_void_p, "temperature top_k top_p min_p u ids logprobs"))
+
+
 def config(vocab, d_model, n_layers, n_heads, n_kv, head_dim, d_ff, max_seq, rope_base=10000.0,
            eps=1e-5) -> LlmqConfig:
     return LlmqConfig(vocab, d_model, n_layers, n_heads, n_kv, head_dim, d_ff, max_seq, rope_base, eps)
@@ -152,6 +193,11 @@ SIGNATURES = {
     "q_llama_tp_unique_id": (C.c_int, [C.c_char_p]),
     "q_llama_tp_init": (C.c_int, [C.c_int, C.c_int, C.c_char_p]),
     "q_llama_tp_shutdown": (None, []),
+    "llmq_paged_plan": (C.c_int, [C.POINTER(PagedPlan), C.c_void_p]),
+    "llmq_paged_append": (C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAppend), C.c_void_p]),
+    "llmq_paged_attention": (C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAttention), C.c_void_p]),
+    "llmq_paged_attention_workspace": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "llmq_sample_rows": (C.c_int, [C.POINTER(SampleRows), C.c_void_p]),
     "q_llama_prefill_argmax": (C.c_int, [C.POINTER(QLlamaModel), C.POINTER(LlamaKV), c_int_p, C.c_int,
                                          C.POINTER(Tensor)]),
 }
