@@ -622,9 +622,11 @@ int llmq_paged_append(const LlmqPagedKV *kv, const LlmqPagedAppend *a, void *str
  *   out = sum_p exp(s_p - m) v_p / sum_p exp(s_p - m),  s_p = scale * <q, k_p>
  * and lse[r][h] = m + log sum_p exp(s_p - m).  n_heads / n_kv query heads share
  * a KV head.  q is in dtype; the pool has the same type, or any type when dtype
- * is LLMQ_F32.  Scores, maxima, sums and the output are formed in f32 and
- * rounded once; with a 16-bit dtype the weights are rounded to it before they
- * multiply the values.  A row without positions gives zeros and lse -infinity.
+ * is LLMQ_F32.  Products are exact, scores, maxima, sums and the output are
+ * formed in f32 and rounded once; over a 16-bit pool the weights multiply the
+ * values as sums of 16-bit terms (16 bits of a weight for bf16 rows, 22 for f16
+ * pools, 24 for f32 rows over bf16).  The result depends on the batch only in
+ * the order of its sums.  A row without positions gives zeros and lse -infinity.
  * Positions on a page outside the pool are left out.  What the pool holds past
  * a row's length is never read into a result.  scale 0 stands for
  * 1 / sqrt(head_dim).  The workspace need not be initialised; calls that may

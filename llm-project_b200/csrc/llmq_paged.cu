@@ -7,7 +7,7 @@
 #include <cmath>
 #include <type_traits>
 
-#include "llmq_serve.cuh"
+#include "llmq_paged_attend.cuh"
 
 using namespace llmq;
 
@@ -225,94 +225,6 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const AppendArgs p, i
   }
 }
 
-// =============================================================== attention
-struct AttendArgs {
-  LlmqPagedKV kv;
-  LlmqPagedAttention a;
-};
-
-constexpr int kAttendWarps = 4;
-
-// One CTA a (row, KV head, query head of its group): the warps share out the
-// positions, a lane owns the dims lane, lane + 32, ...; each warp keeps its own
-// running maximum and sum, joined at the end in shared memory.
-template <typename T, typename KT>
-__global__ void __launch_bounds__(kAttendWarps * 32) k_attend_plain(const AttendArgs p) {
-  constexpr int kPer = 8;  // dims a lane, head_dim <= 256
-  __shared__ float s_o[kAttendWarps][256];
-  __shared__ float s_m[kAttendWarps], s_l[kAttendWarps];
-  serve_wait();
-  serve_dependents();
-  const LlmqPagedKV &kv = p.kv;
-  const LlmqPagedAttention &a = p.a;
-  const int r = blockIdx.y, h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = kv.head_dim;
-  const int kvh = h / (a.n_heads / kv.n_kv);
-  const int seq = a.seqs ? a.seqs[r] : r;
-  long long n = a.lens[r];
-  const long long cap = (long long)a.max_pages * kv.page_size;
-  int flags = 0;
-  if (n < 0 || n > cap || ((seq < 0 || seq >= a.n_seqs) && n > 0)) {
-    flags |= LLMQ_PAGED_BAD_LEN;
-    n = seq < 0 || seq >= a.n_seqs || n < 0 ? 0 : cap;
-  }
-  const long long n0 = a.window > 0 && n > a.window ? n - a.window : 0;
-  const T *q = static_cast<const T *>(a.q) + r * a.q_stride + (size_t)h * hd;
-  float qv[kPer], o[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int d = lane + 32 * i;
-    qv[i] = d < hd ? to_f32(q[d]) : 0.0f;
-    o[i] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (long long pos = n0 + warp; pos < n; pos += kAttendWarps) {
-    const int page = a.table[seq * a.table_stride + pos / kv.page_size];
-    if (page < 0 || page >= kv.n_pages) {
-      flags |= LLMQ_PAGED_BAD_PAGE;
-      continue;
-    }
-    const long long at = page * kv.page_stride + (pos % kv.page_size) * kv.token_stride + kvh * kv.head_stride;
-    const KT *k = static_cast<const KT *>(kv.k) + at, *v = static_cast<const KT *>(kv.v) + at;
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int d = lane + 32 * i;
-      if (d < hd) s = fmaf(qv[i], to_f32(k[d]), s);
-    }
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= a.scale;
-    const float mn = fmaxf(m, s);
-    const float c = m == -INFINITY ? 0.0f : expf(m - mn), e = mn == -INFINITY ? 0.0f : expf(s - mn);
-    l = l * c + e;
-    m = mn;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int d = lane + 32 * i;
-      if (d < hd) o[i] = fmaf(e, to_f32(v[d]), o[i] * c);
-    }
-  }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (lane + 32 * i < hd) s_o[warp][lane + 32 * i] = o[i];
-  if (flags && lane == 0 && a.status) atomicOr(a.status, flags);
-  __syncthreads();
-  float mx = -INFINITY, sum = 0.0f;
-  for (int w = 0; w < kAttendWarps; ++w) mx = fmaxf(mx, s_m[w]);
-  for (int w = 0; w < kAttendWarps; ++w) sum += mx == -INFINITY ? 0.0f : s_l[w] * expf(s_m[w] - mx);
-  T *out = static_cast<T *>(a.out) + r * a.out_stride + (size_t)h * hd;
-  for (int d = threadIdx.x; d < hd; d += kAttendWarps * 32) {
-    float v = 0.0f;
-    for (int w = 0; w < kAttendWarps; ++w) v += mx == -INFINITY ? 0.0f : s_o[w][d] * expf(s_m[w] - mx);
-    out[d] = from_f32<T>(sum > 0.0f ? v / sum : 0.0f);
-  }
-  if (threadIdx.x == 0 && a.lse) a.lse[(size_t)r * a.n_heads + h] = sum > 0.0f ? mx + logf(sum) : -INFINITY;
-}
-
 // ------------------------------------------------------------- host checks
 void check_pool(ServeCheck &c, const LlmqPagedKV *kv) {
   c.require(kv != nullptr, "null pool");
@@ -385,9 +297,47 @@ cudaError_t launch_append(const AppendArgs &p, cudaStream_t st) {
              : serve_launch(k_append<T, KT, 1>, grid, dim3(kAppendThreads), 0, st, p, chunks, lanes);
 }
 
+template <typename Core, int HDP>
+cudaError_t launch_attend(AttendArgs p, int sms, cudaStream_t st) {
+  typedef AttendShape<Core, HDP> Sh;
+  const LlmqPagedAttention &a = p.a;
+  const int group = a.n_heads / p.kv.n_kv, total_rows = a.n_rows;
+  p.blocks = (group + Core::kBlock - 1) / Core::kBlock;
+  cudaError_t e = cudaFuncSetAttribute(k_attend<Core, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+  for (p.row0 = 0; p.row0 < total_rows && e == cudaSuccess; p.row0 += kAttendMaxRows) {
+    p.rows = std::min(kAttendMaxRows, total_rows - p.row0);
+    // no more CTAs than tiles there can be
+    const long long tiles = (long long)p.rows * p.kv.n_kv * p.blocks *
+                            (((long long)a.max_pages * p.kv.page_size + Sh::kTile - 1) / Sh::kTile);
+    const int ctas = static_cast<int>(
+        std::max(1LL, std::min<long long>({tiles, (long long)sms * Sh::kPerSm, (long long)kAttendMaxCtas})));
+    e = serve_launch(k_attend<Core, HDP>, dim3(ctas), dim3(kAttendThreads), Sh::kSmem, st, p);
+    if (e == cudaSuccess && ctas > 1)
+      e = serve_launch(k_attend_join<typename Core::Row>, dim3(ctas, std::min(group, (int)Core::kBlock)), dim3(128), 0,
+                       st, p, ctas, (int)Core::kBlock);
+  }
+  return e;
+}
+
 template <typename T, typename KT>
-cudaError_t launch_attend(const AttendArgs &p, cudaStream_t st) {
-  return serve_launch(k_attend_plain<T, KT>, dim3(p.a.n_heads, p.a.n_rows), dim3(kAttendWarps * 32), 0, st, p);
+cudaError_t attend_by_shape(const AttendArgs &p, int sms, cudaStream_t st) {
+  const int hd = p.kv.head_dim;
+  if constexpr (std::is_same<KT, float>::value) {
+    const int group = p.a.n_heads / p.kv.n_kv;
+    if (group <= 4) {
+      if (hd <= 64) return launch_attend<CoreF32<64, 4>, 64>(p, sms, st);
+      if (hd <= 128) return launch_attend<CoreF32<128, 4>, 128>(p, sms, st);
+      return launch_attend<CoreF32<256, 4>, 256>(p, sms, st);
+    }
+    if (hd <= 64) return launch_attend<CoreF32<64, 8>, 64>(p, sms, st);
+    if (hd <= 128) return launch_attend<CoreF32<128, 8>, 128>(p, sms, st);
+    return launch_attend<CoreF32<256, 8>, 256>(p, sms, st);
+  } else {
+    if (hd <= 64) return launch_attend<CoreMma<T, KT, 64>, 64>(p, sms, st);
+    if (hd <= 96) return launch_attend<CoreMma<T, KT, 96>, 96>(p, sms, st);
+    if (hd <= 128) return launch_attend<CoreMma<T, KT, 128>, 128>(p, sms, st);
+    return launch_attend<CoreMma<T, KT, 256>, 256>(p, sms, st);
+  }
 }
 
 // f(T, KT) for a type of the rows and one of the pool that check_types let through.
@@ -454,7 +404,7 @@ extern "C" LLMQ_API size_t llmq_paged_attention_workspace(int n_rows, int n_head
                    n_heads, n_kv, head_dim);
     return 0;
   }
-  return 16;
+  return attend_workspace(head_dim);
 }
 
 extern "C" LLMQ_API int llmq_paged_attention(const LlmqPagedKV *kv, const LlmqPagedAttention *a, void *stream) {
@@ -469,7 +419,6 @@ extern "C" LLMQ_API int llmq_paged_attention(const LlmqPagedKV *kv, const LlmqPa
   c.require(a->table_stride >= a->max_pages, "table_stride is below max_pages");
   c.require(std::isfinite(a->scale), "scale is not finite");
   if (c.rc != LLMQ_OK || a->n_rows == 0) return c.rc;
-  c.require(a->n_rows <= 65535, "more than 65535 rows");
   c.require(a->q && a->out && a->lens && (a->table || a->max_pages == 0 || a->n_seqs == 0), "null pointer");
   c.require(a->seqs || a->n_seqs >= a->n_rows, "n_seqs is below n_rows and seqs is null");
   const long long qd = (long long)a->n_heads * kv->head_dim;
@@ -492,10 +441,15 @@ extern "C" LLMQ_API int llmq_paged_attention(const LlmqPagedKV *kv, const LlmqPa
   c.memory(a->workspace, "workspace");
   c.memory(a->status, "status");
   if (c.rc != LLMQ_OK) return c.rc;
-  AttendArgs p{*kv, *a};
-  if (p.a.scale == 0.0f) p.a.scale = 1.0f / std::sqrt(static_cast<float>(kv->head_dim));
+  AttendArgs p{};
+  p.kv = *kv;
+  p.a = *a;
+  p.scale_log2 = (a->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(kv->head_dim)) : a->scale) * 1.44269504088896341f;
+  int sms = 0;
+  c.launched(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device));
+  if (c.rc != LLMQ_OK) return c.rc;
   c.launched(by_types(a->dtype, kv->dtype, [&](auto t, auto kt) {
-    return launch_attend<decltype(t), decltype(kt)>(p, static_cast<cudaStream_t>(stream));
+    return attend_by_shape<decltype(t), decltype(kt)>(p, sms, static_cast<cudaStream_t>(stream));
   }));
   return c.rc;
 }

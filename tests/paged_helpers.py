@@ -210,15 +210,18 @@ def attend_plain(k, v, q, table, lens, seqs=None, window=0, scale=0.0):
     return out, lse, bo, bl, vm
 
 
-def check_attend(out, lse, plain, dtype):
-    """The output's rounding adds half a step of its type.  With a 16-bit type the
-    weights are rounded to it: half a step of each weighted value, and as much
-    again through the sum of weights, at most 2 half max|v|."""
+def check_attend(out, lse, plain, dtype, kv_dtype):
+    """The output's rounding adds half a step of its type.  Over a 16-bit pool a weight
+    is a sum of 16-bit terms, off by half a step of the last one: 2^-16 (two bf16
+    terms), 2^-24 (three) or 2^-22 (two of f16) of itself, so the output by that times
+    max|v|."""
     import torch
     o, l, bo, bl, vm = plain
     half = torch.finfo(torch_type(dtype)).eps / 2
+    terms = {"f32": 0.0, "f16": 2.0 ** -22, "bf16": 2.0 ** -24 if dtype == "f32" else 2.0 ** -16}[kv_dtype]
     got, gl = out.double().cpu().numpy(), lse.double().cpu().numpy()
-    tol = bo + half * (np.abs(o) + bo) + (0.0 if dtype == "f32" else 2 * half * vm) + 1e-30
+    tol = bo + terms * vm
+    tol = tol + half * (np.abs(o) + tol) + 1e-30
     assert np.isfinite(got).all()
     off = np.abs(got - o)
     assert (off <= tol).all(), f"{(off > tol).sum()} outputs off, worst {(off / tol).max()} of the bound"

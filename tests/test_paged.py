@@ -81,7 +81,7 @@ def test_append_refuses(lib, bad):
                                  dict(scale=float("inf")), dict(scale=float("nan")), dict(q=None), dict(out=None),
                                  dict(lens=None), dict(table=None), dict(n_seqs=2), dict(q_stride=255),
                                  dict(out_stride=8), dict(q=F + 1), dict(workspace=None), dict(workspace=F + 8),
-                                 dict(workspace_bytes=0), dict(n_rows=65536, n_seqs=65536)], ids=str)
+                                 dict(workspace_bytes=0)], ids=str)
 def test_attention_refuses(lib, bad):
     refused(lib, lib.llmq_paged_attention, pool_args(), attend_args(**bad))
 
@@ -367,7 +367,7 @@ def run_attend(lib, st, dtype, kv_dtype, **kw):
     kw.pop("stream", None)
     if kw.get("seqs") is not None:
         kw["seqs"] = kw["seqs"].cpu()
-    check_attend(out, lse, attend_plain(k, v, q, table, lens, **kw), dtype)
+    check_attend(out, lse, attend_plain(k, v, q, table, lens, **kw), dtype, kv_dtype)
     return out, lse, flags
 
 
@@ -419,7 +419,7 @@ def test_attention_never_reads_past_a_row(lib, dtype, kv_dtype):
         x.copy_(y)
     table[table < 0] = 2 ** 30
     out, lse, flags = attend_gpu(lib, k, v, kv_dtype, q, table, lens, dtype)
-    check_attend(out, lse, want, dtype)
+    check_attend(out, lse, want, dtype, kv_dtype)
     assert flags == 0
 
 
@@ -484,7 +484,7 @@ def test_attention_strided_rows_and_rows_behind(lib, dtype, kv_dtype):
     kv = describe_pool(k, v, kv_dtype)
     ok(lib, lib.llmq_paged_attention(C.byref(kv), C.byref(a), None))
     torch.cuda.synchronize()
-    check_attend(ov, lse[:3], attend_plain(k, v, q, table, lens), dtype)
+    check_attend(ov, lse[:3], attend_plain(k, v, q, table, lens), dtype, kv_dtype)
     assert (wide[3:] == 5).all() and (wide[:, :1] == 5).all() and (wide[:, 257:] == 5).all() and (lse[3:] == 5).all()
 
 
@@ -505,7 +505,7 @@ def test_attention_offsets_past_32_bits(lib, kv_dtype):
     out, lse, flags = attend_gpu(lib, pool, pool, kv_dtype, q, table, lens, "f32")
     small = pool[used].clone()
     want = attend_plain(small, small, q, torch.arange(6)[None].int(), lens)
-    check_attend(out, lse, want, "f32")
+    check_attend(out, lse, want, "f32", kv_dtype)
     assert flags == 0
 
 
@@ -600,5 +600,5 @@ def test_steps_in_a_captured_graph(lib, dtype, kv_dtype):
         assert lens.tolist() == total.tolist() and int(status) == 0 and int(head) == sum(-(-x // page) for x in total)
         s = dict(qkv=qkv, n_kv=KV, heads=H, hd=hd, k=k, v=v, q_out=q, cos=cos, sin=sin, slots=slots, positions=pos)
         check_append(s, append_plain(s))
-        check_attend(out, lse, attend_plain(k, v, q, table, spans, seqs=seqs.cpu()), dtype)
+        check_attend(out, lse, attend_plain(k, v, q, table, spans, seqs=seqs.cpu()), dtype, kv_dtype)
         assert (out[n:] == 0).all() and sorted(set(seqs[:n].tolist())) == [b for b in range(B) if add[b]]
