@@ -3,23 +3,44 @@
 // (llmq_sample_rows).
 //
 // A row's weights are w_j = exp((l_j - max l) / T), as 64-bit integers: w_j is
-// rounded to a whole number of 2^-S, S = 62 - ceil(log2 vocab), so any sum
-// of them is exact, fits 63 bits and is the same in any order.  The tokens'
-// order is the logit's bits mapped to an unsigned key of the same order (key 0:
-// NaN and -infinity, never drawn), then the index.  Each of the three cuts keeps
-// a prefix of that order, so what is kept is known by its sum alone; the draw is
-// the first token at which the sum reaches u times the kept one.
+// rounded to a whole number of 2^-S, S = min(50, 62 - ceil(log2 vocab)), so any
+// sum of them is exact, fits 63 bits and is the same in any order.  The tokens'
+// order is ord = (the logit's bits mapped to an unsigned key of the same order) *
+// 2^20 + 2^20 - 1 - index, larger first (key 0: NaN and -infinity, never drawn).
+// Each of the three cuts keeps a prefix of that order, so what is kept is known
+// by its sum alone, and the draw is the first token at which the sum reaches u
+// times the kept one.  No cut needs a sorted row: only the tokens around it.
+//
+// A cluster of CTAs holds a row in shared memory, read from DRAM once:
+//  1. The largest and least logit, and for a small top_k the largest of each of
+//     some thousand groups of tokens: the k-th largest of those is a bound that at
+//     least k tokens reach and few more do (k = 40: about 41 of a smooth row's).  A
+//     min_p gives another bound.
+//  2. With a bound, the tokens that reach it go to the first CTA's list (the whole
+//     sum, where top_p asks for it, is formed on the way).  The list is sorted and
+//     everything follows from its prefix sums.
+//  3. Without one (or if the list overflows), a histogram of counts and exact
+//     sums over kBins steps of the logit; each cut, then the draw, finds its step by
+//     a prefix sum and lists that step's tokens alone.  A step with too many tokens
+//     is divided again, by ord, down to single tokens if need be (rows of ties).
 #include <climits>
 #include <cmath>
+#include <cooperative_groups.h>
 
 #include "llmq_serve.cuh"
 
 using namespace llmq;
+namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 1024;
 typedef unsigned long long u64;
+constexpr int kThreads = 512;
+constexpr int kBins = 1024;
+constexpr int kListCap = 2048;
+constexpr int kMaxCluster = 8;
+constexpr int kGroups = 2048;  // groups of tokens whose maxima bound a top_k
+constexpr int kIndexBits = 20;
 
 __device__ __forceinline__ uint32_t order_key(float l) {
   const uint32_t b = __float_as_uint(__fadd_rn(l, 0.0f));  // -0 to +0: equal logits, equal keys
@@ -29,67 +50,104 @@ __device__ __forceinline__ uint32_t order_key(float l) {
 __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
+__device__ __forceinline__ u64 token_ord(uint32_t key, int j) {
+  return (static_cast<u64>(key) << kIndexBits) | static_cast<u64>((1 << kIndexBits) - 1 - j);
+}
 
+// exp on the way to an integer: 2^(-y / 64) for y = (max - l) * 64 log2(e) / T as
+// 2^-(n / 64) from a table, 2^-(n % 64 / 64), times the Taylor polynomial of
+// exp(-x), x = (y - n) ln 2 / 64, |x| < 0.0055, up to x^5 (the rest: 2^-54).
 struct RowRule {
-  float mx;       // the largest logit
-  double inv_t;
-  double one;     // 2^S
-  // w of a token that is not excluded (0 beside an infinite maximum, whatever T)
+  float mx;            // the largest logit
+  double mxd, step;    // step: 64 log2(e) / T
+  int scale;           // S
+  const double *tab;   // shared: 2^(-i / 64)
+  float bin_scale;     // steps of the histogram a unit of logit
+
+  // w * 2^S before rounding, for a token that is not excluded (0 beside an
+  // infinite maximum, whatever T)
   __device__ __forceinline__ double share(float l) const {
-    return l == mx ? 1.0 : mx == INFINITY ? 0.0 : exp((static_cast<double>(l) - static_cast<double>(mx)) * inv_t);
+    const double y = (mxd - static_cast<double>(l)) * step;
+    if (!(y < 4032.0)) return l == mx ? __longlong_as_double(static_cast<long long>(1023 + scale) << 52) : 0.0;
+    const double yr = y + 6755399441055744.0;  // 1.5 * 2^52: the integer in the low bits
+    const int n = __double2loint(yr);
+    const double x = (y - (yr - 6755399441055744.0)) * 0.010830424696249145;  // ln 2 / 64
+    double p = fma(x, -1.0 / 120.0, 1.0 / 24.0);
+    p = fma(x, p, -1.0 / 6.0);
+    p = fma(x, p, 0.5);
+    p = fma(x, p, -1.0);
+    p = fma(x, p, 1.0);
+    const double t = tab[n & 63];
+    return p * __hiloint2double(__double2hiint(t) + ((scale - (n >> 6)) << 20), __double2loint(t));
   }
-  __device__ __forceinline__ u64 weight(float l) const {
-    return __double2ull_rn(share(l) * one);
+  static __device__ __forceinline__ u64 round(double s) {
+    const double r = s + 6755399441055744.0;  // s < 2^51
+    return static_cast<u64>(__double_as_longlong(r)) - 0x4338000000000000ull;
+  }
+  __device__ __forceinline__ u64 weight(float l) const { return round(share(l)); }
+  // the histogram's step: any function that does not fall as l falls will do
+  __device__ __forceinline__ int bin(float l) const {
+    const float d = mx - l;
+    if (l == mx) return 0;
+    const float x = d * bin_scale;
+    return x < kBins - 1 ? static_cast<int>(x) : kBins - 1;
   }
 };
 
-template <typename V>
-__device__ __forceinline__ V block_sum(V v, V *red) {
+struct Command {
+  int op;           // what the cluster does next
+  int bin0, bin1;   // tokens of these steps
+  u64 lo, hi;       // and of this range of ord
+  int shift;        // op kDivide: the new step is (hi - ord) >> shift
+};
+enum { kDone = 0, kGather = 1, kDivide = 2 };
+
+// What each CTA keeps in static shared memory; the first CTA's is the row's.
+struct Shared {
+  double tab[64];
+  u64 red[kThreads / 32];
+  u64 top[kMaxCluster], whole[kMaxCluster], above[kMaxCluster];
+  uint32_t least[kMaxCluster];
+  int listed;        // tokens gathered here
+  int total;         // the row's list (first CTA)
+  int place;         // where this CTA's part of it goes
+  unsigned digits[256];
+  uint32_t pick_key;
+  int pick_bin, pick_count;
+  u64 pick_before, pick_before_count;
+  int pick_item;
+  Command cmd;
+};
+
+__device__ __forceinline__ u64 warp_scan(u64 v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += u;
+  }
+  return v;
+}
+// Inclusive sum over the block's threads; every thread of the block calls this.
+__device__ __forceinline__ u64 block_scan(u64 v, u64 *red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_scan(v);
+  __syncthreads();
+  if (lane == 31) red[warp] = v;
+  __syncthreads();
+  const u64 w = warp_scan(lane < kThreads / 32 ? red[lane] : 0);
+  const u64 before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return warp ? v + before : v;
+}
+__device__ __forceinline__ u64 block_sum(u64 v, u64 *red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = red[threadIdx.x & 31];
+  v = red[threadIdx.x & (kThreads / 32 - 1)];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = kThreads / 64; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
-}
-
-struct Found {
-  uint32_t key;
-  u64 before;  // measure of the tokens with larger keys
-};
-
-// The key at which the measure (1 or w of each token, over falling keys) reaches
-// `target` (1 .. the row's whole measure): four levels of 256 bins.
-template <bool mass, typename T>
-__device__ Found reach(const T *row, int V, const RowRule &rule, u64 target, u64 *bins, u64 *pick) {
-  uint32_t prefix = 0u, mask = 0u;
-  u64 before = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    for (int b = threadIdx.x; b < 256; b += kThreads) bins[b] = 0;
-    __syncthreads();
-    for (int j = threadIdx.x; j < V; j += kThreads) {
-      const float l = to_f32(row[j]);
-      const uint32_t k = order_key(l);
-      if (k != 0u && (k & mask) == prefix) atomicAdd(&bins[(k >> shift) & 255u], mass ? rule.weight(l) : 1ull);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int b = 255;
-      u64 sum = before;
-      for (; b > 0 && sum + bins[b] < target; --b) sum += bins[b];
-      pick[0] = b;
-      pick[1] = sum;
-    }
-    __syncthreads();
-    prefix |= static_cast<uint32_t>(pick[0]) << shift;
-    before = pick[1];
-    mask |= 255u << shift;
-  }
-  return Found{prefix, before};
 }
 
 // ceil(f * total) in 1 .. total
@@ -99,117 +157,614 @@ __device__ __forceinline__ u64 part_of(double f, u64 total) {
   return v > total ? total : v;
 }
 
+// Dynamic shared memory: the histogram (counts, then the sums' low and high
+// words) or this CTA's gathered tokens; the row's histogram; the row's list or
+// the histogram of a divided step; the slice of the row.
+constexpr int kHistBytes = kBins * 12;
+constexpr int kListBytes = kListCap * 8;
+constexpr int kWorkBytes = kListBytes + kHistBytes + kListBytes;
+static_assert(kHistBytes <= kListBytes && kGroups * 4 <= kHistBytes, "regions are shared");
+
+struct RowArgs {
+  LlmqSampleRows a;
+  int slice;     // tokens a CTA, a multiple of 16
+  int resident;  // the slice is kept in shared memory
+  int scale;     // S
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_sample_rows(const LlmqSampleRows a, int bits) {
-  __shared__ u64 s_bins[256], s_red[32], s_pick[2];
-  __shared__ uint32_t s_key[32];
-  __shared__ int s_idx[32];
+__global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
+  extern __shared__ __align__(16) unsigned char s_dyn[];
+  __shared__ Shared sh;
+  constexpr int kVec = 16 / sizeof(T);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  uint32_t *bin_count = reinterpret_cast<uint32_t *>(s_dyn), *bin_lo = bin_count + kBins, *bin_hi = bin_lo + kBins;
+  u64 *gathered = reinterpret_cast<u64 *>(s_dyn);
+  u64 *tot_mass = reinterpret_cast<u64 *>(s_dyn + kListBytes);
+  uint32_t *tot_count = reinterpret_cast<uint32_t *>(tot_mass + kBins);
+  u64 *list = reinterpret_cast<u64 *>(s_dyn + kListBytes + kHistBytes);
+  uint32_t *groups = reinterpret_cast<uint32_t *>(tot_mass);  // read before any CTA can be at a histogram's sums
+  T *slice = reinterpret_cast<T *>(s_dyn + kWorkBytes);
+  Shared *first = cluster.map_shared_rank(&sh, 0);
+
+  const LlmqSampleRows &a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = blockIdx.x / ctas, j0 = rank * p.slice, n = max(0, min(p.slice, a.vocab - j0));
+  cluster.barrier_arrive();  // every CTA runs before any writes to another
+  if (tid < 64) sh.tab[tid] = exp2(-tid / 64.0);
+  if (tid == 0) sh.listed = sh.total = 0;
   serve_wait();
   serve_dependents();
-  const int r = blockIdx.x, V = a.vocab, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T *row = static_cast<const T *>(a.logits) + r * a.stride;
-  // the first largest logit
-  uint32_t best = 0u;
-  int at = INT_MAX;
-  for (int j = tid; j < V; j += kThreads) {
-    const uint32_t k = order_key(to_f32(row[j]));
-    if (k > best) {
-      best = k;
-      at = j;
-    }
-  }
-  auto better = [&](uint32_t k, int i) {
-    if (k > best || (k == best && i < at)) {
-      best = k;
-      at = i;
+  const T *row = static_cast<const T *>(a.logits) + r * a.stride + j0;
+  const float temp = a.temperature ? a.temperature[r] : 1.0f;
+  const bool greedy = !(temp > 0.0f);
+  const float min_p = a.min_p && a.min_p[r] > 0.0f ? fminf(a.min_p[r], 1.0f) : 0.0f;
+  const float top_p = a.top_p && a.top_p[r] > 0.0f && a.top_p[r] < 1.0f ? a.top_p[r] : 0.0f;
+  const int top_k = a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.vocab ? a.top_k[r] : 0;
+
+  // f(logit, index) for every token of the slice
+  auto each = [&](auto f) {
+    if (p.resident) {
+      for (int v = tid; v < (n + kVec - 1) / kVec; v += kThreads) {
+        const Pack<T, kVec> x = reinterpret_cast<const Pack<T, kVec> *>(slice)[v];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) f(to_f32(x.v[i]), j0 + v * kVec + i);
+      }
+    } else {
+      for (int j = tid; j < n; j += kThreads) f(to_f32(row[j]), j0 + j);
     }
   };
+
+  // ---- 1. the slice, its largest (with its first index) and least logit
+  if (p.resident) {
+    if ((reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+#pragma unroll 4
+      for (int v = tid; v < n / kVec; v += kThreads)
+        reinterpret_cast<Pack<T, kVec> *>(slice)[v] = reinterpret_cast<const Pack<T, kVec> *>(row)[v];
+      for (int j = n / kVec * kVec + tid; j < n; j += kThreads) slice[j] = row[j];
+    } else {
+#pragma unroll 4
+      for (int j = tid; j < n; j += kThreads) slice[j] = row[j];
+    }
+    for (int j = n + tid; j < (n + kVec - 1) / kVec * kVec; j += kThreads) slice[j] = from_f32<T>(-INFINITY);
+    __syncthreads();
+  }
+  u64 best = 0;            // the largest ord (0: none)
+  uint32_t least = ~0u;    // the least key
+  each([&](float l, int j) {
+    const uint32_t k = order_key(l);
+    const u64 o = token_ord(k, j);
+    best = k && o > best ? o : best;
+    least = k ? min(least, k) : least;
+  });
+  const int group_threads = max(1, ctas * kThreads / kGroups), cta_groups = kThreads / group_threads;
+  {
+    uint32_t g = static_cast<uint32_t>(best >> kIndexBits);
+    for (int o = 1; o < group_threads; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+    u64 b = best;
+    uint32_t lo = least;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint32_t k = __shfl_xor_sync(0xffffffffu, best, o);
-    const int i = __shfl_xor_sync(0xffffffffu, at, o);
-    better(k, i);
+    for (int o = 16; o > 0; o >>= 1) {
+      const u64 u = __shfl_xor_sync(0xffffffffu, b, o);
+      b = u > b ? u : b;
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    }
+    if (lane == 0) {
+      sh.red[warp] = b;
+      sh.digits[warp] = lo;
+    }
+    __syncthreads();
+    cluster.barrier_wait();
+    if (top_k && !greedy && tid % group_threads == 0)
+      for (int c = 0; c < ctas; ++c)
+        cluster.map_shared_rank(groups, c)[rank * cta_groups + tid / group_threads] = g;
+    if (tid < ctas) {
+      u64 m = 0;
+      uint32_t lw = ~0u;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        m = sh.red[w] > m ? sh.red[w] : m;
+        lw = min(lw, sh.digits[w]);
+      }
+      Shared *to = cluster.map_shared_rank(&sh, tid);
+      to->top[rank] = m;
+      to->least[rank] = lw;
+    }
   }
-  if (lane == 0) {
-    s_key[warp] = best;
-    s_idx[warp] = at;
+  cluster.sync();
+  u64 top = 0;
+  uint32_t low = ~0u;
+  for (int c = 0; c < ctas; ++c) {
+    top = sh.top[c] > top ? sh.top[c] : top;
+    low = min(low, sh.least[c]);
   }
-  __syncthreads();
-  for (int w = 0; w < 32; ++w) better(s_key[w], s_idx[w]);
-  const float temp = a.temperature ? a.temperature[r] : 1.0f;
-  if (best == 0u || !(temp > 0.0f)) {
-    if (tid == 0) {
-      a.ids[r] = best == 0u ? -1 : at;
-      if (a.logprobs) a.logprobs[r] = best == 0u ? -INFINITY : 0.0f;
+  if (top == 0 || greedy) {
+    if (rank == 0 && tid == 0) {
+      a.ids[r] = top == 0 ? -1 : (1 << kIndexBits) - 1 - static_cast<int>(top & ((1 << kIndexBits) - 1));
+      if (a.logprobs) a.logprobs[r] = top == 0 ? -INFINITY : 0.0f;
     }
     return;
   }
-  RowRule rule{key_logit(best), 1.0 / static_cast<double>(temp), ldexp(1.0, bits)};
-  const float min_p = a.min_p && a.min_p[r] > 0.0f ? fminf(a.min_p[r], 1.0f) : 0.0f, top_p = a.top_p ? a.top_p[r] : 0.0f;
-  const int top_k = a.top_k ? a.top_k[r] : 0;
-  // the whole sum, the sum of w >= min_p, the number of tokens that can be drawn
-  u64 whole = 0, above = 0, count = 0;
-  for (int j = tid; j < V; j += kThreads) {
-    const float l = to_f32(row[j]);
-    if (order_key(l) == 0u) continue;
-    const double e = rule.share(l);
-    const u64 w = __double2ull_rn(e * rule.one);
-    whole += w;
-    above += min_p > 0.0f && !(e >= static_cast<double>(min_p)) ? 0 : w;
-    ++count;
+  RowRule rule;
+  rule.mx = key_logit(static_cast<uint32_t>(top >> kIndexBits));
+  rule.mxd = static_cast<double>(rule.mx);
+  rule.step = 64.0 * 1.4426950408889634 / static_cast<double>(temp);
+  rule.scale = p.scale;
+  rule.tab = sh.tab;
+  {
+    // steps over what the row spans, or down to weights that round to nothing
+    const float span = fminf(rule.mx - key_logit(low), 36.0f * temp);
+    rule.bin_scale = span > 0.0f && span < INFINITY ? kBins / span : 0.0f;
   }
-  whole = block_sum(whole, s_red);
-  above = block_sum(above, s_red);
-  count = block_sum(count, s_red);
-  u64 kept = above;
-  if (top_k > 0 && static_cast<u64>(top_k) < count) {
-    const Found f = reach<false>(row, V, rule, top_k, s_bins, s_pick);
-    u64 sum = 0;
-    for (int j = tid; j < V; j += kThreads) {
-      const float l = to_f32(row[j]);
-      if (order_key(l) > f.key) sum += rule.weight(l);
+
+  // ---- a bound that the tokens of every cut reach
+  uint32_t bound = 0;
+  bool bounded = a.vocab <= kListCap;
+  if (!bounded && top_k && top_k <= ctas * cta_groups * 3 / 4) {
+    // the top_k-th largest of the groups' maxima, by digits of 8 bits
+    const int ng = ctas * cta_groups;
+    uint32_t prefix = 0, mask = 0;
+    int rest = top_k;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) sh.digits[tid] = 0;
+      __syncthreads();
+      for (int i = tid; i < ng; i += kThreads)
+        if ((groups[i] & mask) == prefix) atomicAdd(&sh.digits[(groups[i] >> shift) & 255u], 1u);
+      __syncthreads();
+      if (warp == 0) {
+        // lane: digits 255 - 8 lane down to 248 - 8 lane
+        int sum = 0;
+        for (int i = 0; i < 8; ++i) sum += sh.digits[255 - 8 * lane - i];
+        const int incl = static_cast<int>(warp_scan(sum));
+        const unsigned who = __ballot_sync(0xffffffffu, incl >= rest);
+        if (lane == __ffs(who) - 1) {
+          int before = incl - sum, d = 255 - 8 * lane;
+          while (before + static_cast<int>(sh.digits[d]) < rest) before += sh.digits[d--];
+          sh.pick_key = prefix | (static_cast<uint32_t>(d) << shift);
+          sh.pick_count = rest - before;
+        }
+      }
+      __syncthreads();
+      prefix = sh.pick_key;
+      rest = sh.pick_count;
+      mask |= 255u << shift;
     }
-    sum = block_sum(sum, s_red) + (top_k - f.before) * rule.weight(key_logit(f.key));
-    kept = min(kept, sum);
+    bound = prefix;
+    bounded = true;
   }
-  if (top_p > 0.0f && top_p < 1.0f) {
-    const u64 target = part_of(top_p, whole);
-    const Found f = reach<true>(row, V, rule, target, s_bins, s_pick);
-    const u64 w = rule.weight(key_logit(f.key));
-    kept = min(kept, f.before + (target - f.before + w - 1) / w * w);
+  if (min_p > 0.0f) {
+    // l >= max + T ln(min_p), a little lower: the list is cut exactly
+    const double at = rule.mxd + static_cast<double>(temp) * log(static_cast<double>(min_p)) * (1.0 + 1e-6);
+    const uint32_t k = order_key(__double2float_rd(at - 1e-6 * fabs(rule.mxd)));
+    bound = max(bound, min(k, static_cast<uint32_t>(top >> kIndexBits)));
+    bounded = true;
   }
+  __syncthreads();  // the groups have been read
+
+  // ---- 2. the tokens that reach the bound
+  auto gather = [&](auto wanted) {  // into `gathered`, then to the first CTA's list
+    each([&](float l, int j) {
+      const uint32_t k = order_key(l);
+      const bool want = k && wanted(l, k, j);
+      const unsigned bal = __ballot_sync(__activemask(), want);
+      if (want) {
+        const int lead = __ffs(bal) - 1;
+        int at = 0;
+        if (lane == lead) at = atomicAdd(&sh.listed, __popc(bal));
+        at = __shfl_sync(bal, at, lead) + __popc(bal & ((1u << lane) - 1u));
+        if (at < kListCap) gathered[at] = token_ord(k, j);
+      }
+    });
+    __syncthreads();
+    const int mine = sh.listed;
+    if (tid == 0) sh.place = mine ? atomicAdd(&first->total, mine) : 0;
+    __syncthreads();
+    u64 *to = cluster.map_shared_rank(list, 0);
+    for (int i = tid; i < min(mine, kListCap); i += kThreads)
+      if (sh.place + i < kListCap) to[sh.place + i] = gathered[i];
+    if (tid == 0) sh.listed = 0;
+  };
+  const double min_share = ldexp(static_cast<double>(min_p), p.scale);
+  u64 whole = 0, above = 0;
+  if (bounded) {
+    gather([&](float, uint32_t k, int) { return k >= bound; });
+    if (top_p > 0.0f) each([&](float l, int) { whole += l > -INFINITY ? rule.weight(l) : 0; });
+  } else {
+    for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
+    __syncthreads();
+  }
+  auto count_in = [&](uint32_t w_lo, uint32_t w_hi, int b) {
+    atomicAdd(&bin_count[b], 1u);
+    const uint32_t old = atomicAdd(&bin_lo[b], w_lo);
+    w_hi += old + w_lo < old ? 1u : 0u;
+    if (w_hi) atomicAdd(&bin_hi[b], w_hi);
+  };
+  auto histogram = [&]() {
+    each([&](float l, int) {
+      if (!(l > -INFINITY)) return;
+      const double s = rule.share(l);
+      const u64 w = RowRule::round(s);
+      whole += w;
+      above += s >= min_share ? w : 0;
+      count_in(static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32), rule.bin(l));
+    });
+  };
+  // the row's histogram in the first CTA, each CTA summing a part of the steps
+  auto collect = [&](u64 *mass, uint32_t *count) {
+    cluster.sync();
+    const int each_bins = kBins / ctas;
+    u64 *m0 = cluster.map_shared_rank(mass, 0);
+    uint32_t *c0 = cluster.map_shared_rank(count, 0);
+    for (int i = tid; i < each_bins; i += kThreads) {
+      const int b = rank * each_bins + i;
+      u64 m = 0;
+      uint32_t cnt = 0;
+      for (int c = 0; c < ctas; ++c) {
+        const uint32_t *h = cluster.map_shared_rank(bin_count, c);
+        cnt += h[b];
+        m += h[kBins + b] + (static_cast<u64>(h[2 * kBins + b]) << 32);
+      }
+      m0[b] = m;
+      c0[b] = cnt;
+    }
+  };
+  auto publish = [&]() {
+    whole = block_sum(whole, sh.red);
+    above = block_sum(above, sh.red);
+    if (tid == 0) {
+      first->whole[rank] = whole;
+      first->above[rank] = above;
+    }
+  };
+  bool have_hist = false;
+  if (!bounded) {
+    histogram();
+    publish();
+    collect(tot_mass, tot_count);
+    have_hist = true;
+  } else if (top_p > 0.0f) {
+    publish();
+  }
+  cluster.sync();
+  if (bounded) {
+    const bool overflow = first->total > kListCap;
+    cluster.barrier_arrive();  // the first CTA outlives the others' look at its memory
+    if (overflow) {  // too many reach the bound: by the histogram after all
+      cluster.barrier_wait();
+      whole = above = 0;
+      for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
+      __syncthreads();
+      histogram();
+      publish();
+      collect(tot_mass, tot_count);
+      have_hist = true;
+      cluster.sync();
+    } else if (rank != 0) {
+      return;
+    }
+  }
+
+  // ---- the first CTA decides, the others gather and divide as it says
+  // sorts list[0 .. m) by falling ord, m <= kListCap
+  auto sort_list = [&](int m) {
+    int size2 = 2;
+    while (size2 < m) size2 <<= 1;
+    for (int i = m + tid; i < size2; i += kThreads) list[i] = 0;
+    __syncthreads();
+    for (int size = 2; size <= size2; size <<= 1)
+      for (int stride = size >> 1; stride > 0; stride >>= 1) {
+        for (int i = tid; i < size2 / 2; i += kThreads) {
+          const int x = 2 * i - (i & (stride - 1)), y = x + stride;
+          const u64 u = list[x], v = list[y];
+          if ((u < v) == ((x & size) == 0)) {
+            list[x] = v;
+            list[y] = u;
+          }
+        }
+        __syncthreads();
+      }
+  };
+  constexpr int kPer = kListCap / kThreads;
+  // the sorted list's sums: thread's items tid * kPer + i, sum up to and with each
+  auto list_sums = [&](int m, u64 before, u64 *sums) {
+    u64 w[kPer], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int x = tid * kPer + i;
+      w[i] = x < m ? rule.weight(key_logit(static_cast<uint32_t>(list[x] >> kIndexBits))) : 0;
+      mine += w[i];
+    }
+    u64 at = before + block_scan(mine, sh.red) - mine;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      at += w[i];
+      sums[i] = at;
+    }
+  };
+  // the first of the list's items whose sum reaches target (there is one), and its sum
+  auto reach = [&](int m, const u64 *sums, u64 target, u64 *sum_there) {
+    __syncthreads();
+    if (tid == 0) sh.pick_item = INT_MAX;
+    __syncthreads();
+#pragma unroll
+    for (int i = kPer - 1; i >= 0; --i) {
+      const int x = tid * kPer + i;
+      if (x < m && sums[i] >= target) atomicMin(&sh.pick_item, x);
+    }
+    __syncthreads();
+    const int item = min(sh.pick_item, m - 1);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (tid * kPer + i == item) sh.pick_before = sums[i];
+    __syncthreads();
+    *sum_there = sh.pick_before;
+    return item;
+  };
+  auto answer = [&](int item, u64 kept) {
+    if (tid == 0) {
+      const u64 o = list[item];
+      const float l = key_logit(static_cast<uint32_t>(o >> kIndexBits));
+      a.ids[r] = (1 << kIndexBits) - 1 - static_cast<int>(o & ((1 << kIndexBits) - 1));
+      if (a.logprobs) {
+        const double lw = l == rule.mx ? 0.0 : -(rule.mxd - static_cast<double>(l)) / static_cast<double>(temp);
+        a.logprobs[r] = static_cast<float>(lw - log(ldexp(static_cast<double>(kept), -p.scale)));
+      }
+    }
+  };
   const float uf = a.u[r];
-  const u64 target = part_of(uf > 0.0f ? fminf(uf, 1.0f) : 0.0f, kept);
-  const Found f = reach<true>(row, V, rule, target, s_bins, s_pick);
-  const float l_at = key_logit(f.key);
-  // among equal logits, the nth by index
-  const u64 nth = (target - f.before + rule.weight(l_at) - 1) / rule.weight(l_at);
-  u64 seen = 0;
-  for (int j0 = 0; j0 < V; j0 += kThreads) {
-    const int j = j0 + tid;
-    const bool same = j < V && order_key(to_f32(row[j])) == f.key;
-    const unsigned bal = __ballot_sync(0xffffffffu, same);
-    __syncthreads();
-    if (lane == 0) s_red[warp] = __popc(bal);
-    __syncthreads();
-    u64 mine = seen;
-    for (int w = 0; w < warp; ++w) mine += s_red[w];
-    mine += __popc(bal & ((1u << lane) - 1u)) + 1;
-    if (same && mine == nth) {
-      a.ids[r] = j;
-      if (a.logprobs)
-        a.logprobs[r] = static_cast<float>(log(rule.share(l_at) * rule.one / static_cast<double>(kept)));
+  const double u = uf > 0.0f ? fminf(uf, 1.0f) : 0.0f;
+
+  if (!have_hist) {  // the list has every cut
+    const int m = sh.total;
+    u64 sums[kPer], there;
+    sort_list(m);
+    list_sums(m, 0, sums);
+    u64 kept = ~0ull;
+    if (top_k && top_k < m) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (tid * kPer + i == top_k - 1) sh.pick_before = sums[i];
+      __syncthreads();
+      kept = sh.pick_before;
     }
-    for (int w = 0; w < 32; ++w) seen += s_red[w];
-    if (seen >= nth) break;
+    {  // the last item, or the last with w >= min_p
+      int last = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int x = tid * kPer + i;
+        if (x < m && rule.share(key_logit(static_cast<uint32_t>(list[x] >> kIndexBits))) >= min_share) last = x + 1;
+      }
+      __syncthreads();
+      if (tid == 0) sh.pick_item = 0;
+      __syncthreads();
+      if (last) atomicMax(&sh.pick_item, last);
+      __syncthreads();
+      const int item = sh.pick_item - 1;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (tid * kPer + i == item) sh.pick_before = sums[i];
+      __syncthreads();
+      kept = min(kept, sh.pick_before);
+    }
+    if (top_p > 0.0f) {
+      u64 z = 0;
+      for (int c = 0; c < ctas; ++c) z += sh.whole[c];
+      const u64 target = part_of(top_p, z);
+      if (target < kept) {  // reached within the list
+        reach(m, sums, target, &there);
+        kept = min(kept, there);
+      }
+    }
+    const int item = reach(m, sums, part_of(u, kept), &there);
+    answer(item, kept);
+    cluster.barrier_wait();
+    return;
   }
+
+  // the tokens of a command's steps and range
+  auto in_command = [&](const Command &c, float l, uint32_t k, int j) {
+    const u64 o = token_ord(k, j);
+    const int b = rule.bin(l);
+    return b >= c.bin0 && b <= c.bin1 && o >= c.lo && o <= c.hi;
+  };
+  auto obey = [&]() -> bool {  // every CTA: false when the row is done
+    cluster.sync();  // the command stands, the list is empty
+    const Command c = first->cmd;
+    if (c.op == kDone) {
+      cluster.sync();  // the first CTA outlives the others' look at its memory
+      return false;
+    }
+    if (c.op == kGather) {
+      gather([&](float l, uint32_t k, int j) { return in_command(c, l, k, j); });
+    } else {
+      for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
+      __syncthreads();
+      each([&](float l, int j) {
+        const uint32_t k = order_key(l);
+        if (!k || !in_command(c, l, k, j)) return;
+        const u64 w = rule.weight(l), s = (c.hi - token_ord(k, j)) >> c.shift;
+        count_in(static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32), static_cast<int>(min(s, (u64)(kBins - 1))));
+      });
+      collect(list, reinterpret_cast<uint32_t *>(list + kBins));
+    }
+    cluster.sync();
+    return true;
+  };
+  if (rank != 0) {
+    while (obey()) {
+    }
+    return;
+  }
+  // The step of `mass` / `count` in which the measure reaches target, from `before`
+  // (sums) and `before_n` (tokens) on.
+  auto find_step = [&](const u64 *mass, const uint32_t *count, bool by_count, u64 target, u64 before, u64 before_n) {
+    u64 m[kBins / kThreads], c[kBins / kThreads], ms = 0, cs = 0;
+#pragma unroll
+    for (int i = 0; i < kBins / kThreads; ++i) {
+      m[i] = mass[tid * (kBins / kThreads) + i];
+      c[i] = count[tid * (kBins / kThreads) + i];
+      ms += m[i];
+      cs += c[i];
+    }
+    u64 am = before + block_scan(ms, sh.red) - ms;
+    u64 ac = before_n + block_scan(cs, sh.red) - cs;
+#pragma unroll
+    for (int i = 0; i < kBins / kThreads; ++i) {
+      const u64 has = by_count ? ac : am, gets = has + (by_count ? c[i] : m[i]);
+      if (has < target && gets >= target) {  // one step of the row
+        sh.pick_bin = tid * (kBins / kThreads) + i;
+        sh.pick_before = am;
+        sh.pick_before_count = ac;
+        sh.pick_count = static_cast<int>(c[i]);
+      }
+      am += m[i];
+      ac += c[i];
+    }
+    __syncthreads();
+  };
+  // Lists the tokens around where the measure reaches target; returns the item there,
+  // *sum_there the row's sum up to and with it.  If all tokens up to there fit the
+  // list, they are listed and *from_start is set.
+  int m = 0;
+  u64 sums[kPer];
+  auto select = [&](bool by_count, u64 target, bool *from_start, u64 *sum_there) {
+    find_step(tot_mass, tot_count, by_count, target, 0, 0);
+    Command c{};
+    c.bin0 = c.bin1 = sh.pick_bin;
+    c.hi = ~0ull;
+    u64 before = sh.pick_before, before_n = sh.pick_before_count;
+    int here = sh.pick_count;
+    *from_start = before_n + here <= kListCap;
+    if (*from_start) {
+      c.bin0 = 0;
+      before = before_n = 0;
+      here = 0;
+    }
+    __syncthreads();
+    // Divide the step by ord until it fits.  ord has 52 bits and each division takes
+    // 10 of them, after a first one by a range estimated from the step's logits (its
+    // last part takes what lies below the estimate): 7 suffice.
+    for (int level = 0; here > kListCap && level < 8; ++level) {
+      if (level == 0) {
+        const float w = rule.bin_scale > 0.0f ? 1.0f / rule.bin_scale : INFINITY;
+        const uint32_t kh = order_key(rule.mx - w * (static_cast<float>(c.bin0) - 0.5f));  // half a step over it
+        const uint32_t kl = order_key(rule.mx - w * static_cast<float>(c.bin0 + 1));
+        c.hi = c.bin0 == 0 || kh == 0 ? top : token_ord(kh, 0);
+        const u64 lo = c.bin0 + 1 == kBins || kl < low ? static_cast<u64>(low) << kIndexBits : token_ord(kl, (1 << kIndexBits) - 1);
+        c.shift = 0;
+        while (c.hi > lo && ((c.hi - lo) >> c.shift) >= kBins) ++c.shift;
+      }
+      c.op = kDivide;
+      if (tid == 0) sh.cmd = c;
+      __syncthreads();
+      obey();
+      find_step(list, reinterpret_cast<const uint32_t *>(list + kBins), by_count, target, before, before_n);
+      const u64 s = sh.pick_bin;
+      before = sh.pick_before;
+      before_n = sh.pick_before_count;
+      here = sh.pick_count;
+      __syncthreads();
+      const u64 hi = c.hi - (s << c.shift);
+      if (s + 1 < kBins) c.lo = hi - ((1ull << c.shift) - 1);
+      c.hi = hi;
+      // the last step runs down to lo
+      const u64 size = c.hi - c.lo;
+      c.shift = 0;
+      while ((size >> c.shift) >= kBins) ++c.shift;
+    }
+    c.op = kGather;
+    if (tid == 0) {
+      sh.cmd = c;
+      sh.total = 0;
+    }
+    __syncthreads();
+    obey();
+    m = min(sh.total, kListCap);
+    sort_list(m);
+    list_sums(m, before, sums);
+    if (by_count) {
+      const int item = min(static_cast<int>(target - before_n) - 1, m - 1);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (tid * kPer + i == item) sh.pick_before = sums[i];
+      __syncthreads();
+      *sum_there = sh.pick_before;
+      return item;
+    }
+    return reach(m, sums, target, sum_there);
+  };
+  u64 z = 0, kept = 0, tokens = 0;
+  for (int c = 0; c < ctas; ++c) {
+    z += sh.whole[c];
+    kept += sh.above[c];
+  }
+  for (int b = tid; b < kBins; b += kThreads) tokens += tot_count[b];
+  tokens = block_sum(tokens, sh.red);
+  bool from_start = false;
+  u64 there;
+  if (top_k && static_cast<u64>(top_k) < tokens) {
+    select(true, top_k, &from_start, &there);
+    kept = min(kept, there);
+  }
+  if (top_p > 0.0f) {
+    const u64 target = part_of(top_p, z);
+    if (target < kept) {
+      if (from_start)
+        reach(m, sums, target, &there);
+      else
+        select(false, target, &from_start, &there);
+      kept = min(kept, there);
+    }
+  }
+  const u64 target = part_of(u, kept);
+  int item;
+  if (from_start)
+    item = reach(m, sums, target, &there);
+  else
+    item = select(false, target, &from_start, &there);
+  answer(item, kept);
+  __syncthreads();
+  if (tid == 0) sh.cmd.op = kDone;
+  __syncthreads();
+  obey();
 }
 
 template <typename T>
-cudaError_t launch(const LlmqSampleRows &a, cudaStream_t st) {
+cudaError_t launch(const LlmqSampleRows &a, int sms, cudaStream_t st) {
+  RowArgs p{};
+  p.a = a;
   int log2v = 0;
   while ((1 << log2v) < a.vocab) ++log2v;
-  return serve_launch(k_sample_rows<T>, dim3(a.n_rows), dim3(kThreads), 0, st, a, 62 - log2v);
+  p.scale = 62 - log2v < 50 ? 62 - log2v : 50;
+  // CTAs a row: a slice of at most 64 KB (two CTAs an SM), more while SMs idle
+  int ctas = 1;
+  auto slice_of = [&](int c) { return ((a.vocab + c - 1) / c + 15) / 16 * 16; };
+  while (ctas < kMaxCluster && (slice_of(ctas) * sizeof(T) > 64 * 1024 ||
+                                ((long long)a.n_rows * ctas < 2 * sms && slice_of(ctas) > 2 * kThreads)))
+    ctas *= 2;
+  p.slice = slice_of(ctas);
+  p.resident = p.slice * sizeof(T) <= 160 * 1024;
+  const int smem = kWorkBytes + (p.resident ? p.slice * (int)sizeof(T) : 0);
+  cudaError_t e = cudaFuncSetAttribute(k_sample_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.n_rows) * ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = ctas;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, k_sample_rows<T>, p);
 }
 
 }  // namespace
@@ -219,8 +774,8 @@ extern "C" LLMQ_API int llmq_sample_rows(const LlmqSampleRows *a, void *stream) 
   c.require(a != nullptr, "null descriptor");
   if (c.rc != LLMQ_OK) return c.rc;
   c.require(serve_dtype(a->dtype), "unknown type of the logits");
-  c.require(a->n_rows >= 0, "negative size");
-  c.require(a->vocab > 0 && a->vocab <= (1 << 20), "vocab outside 1..2^20");
+  c.require(a->n_rows >= 0 && a->n_rows <= INT_MAX / kMaxCluster, "n_rows outside 0..2^28 - 1");
+  c.require(a->vocab > 0 && a->vocab <= (1 << kIndexBits), "vocab outside 1..2^20");
   if (c.rc != LLMQ_OK || a->n_rows == 0) return c.rc;
   c.require(a->logits && a->u && a->ids, "null pointer");
   c.require(a->stride >= a->vocab, "a row stride is shorter than its row");
@@ -235,9 +790,12 @@ extern "C" LLMQ_API int llmq_sample_rows(const LlmqSampleRows *a, void *stream) 
   c.memory(a->ids, "ids");
   c.memory(a->logprobs, "logprobs");
   if (c.rc != LLMQ_OK) return c.rc;
+  int sms = 0;
+  c.launched(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device));
+  if (c.rc != LLMQ_OK) return c.rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  c.launched(a->dtype == LLMQ_F32   ? launch<float>(*a, st)
-             : a->dtype == LLMQ_F16 ? launch<__half>(*a, st)
-                                    : launch<__nv_bfloat16>(*a, st));
+  c.launched(a->dtype == LLMQ_F32   ? launch<float>(*a, sms, st)
+             : a->dtype == LLMQ_F16 ? launch<__half>(*a, sms, st)
+                                    : launch<__nv_bfloat16>(*a, sms, st));
   return c.rc;
 }
