@@ -23,6 +23,7 @@
 //     sums over kBins steps of the logit; each cut, then the draw, finds its step by
 //     a prefix sum and lists that step's tokens alone.  A step with too many tokens
 //     is divided again, by ord, down to single tokens if need be (rows of ties).
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cooperative_groups.h>
@@ -47,6 +48,7 @@ __device__ __forceinline__ uint32_t order_key(float l) {
   if (!(l > -INFINITY)) return 0u;
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
+constexpr uint32_t kKeyNegInf = 0x007fffffu;  // order_key's value for it but for the exclusion
 __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
@@ -106,8 +108,8 @@ enum { kDone = 0, kGather = 1, kDivide = 2 };
 struct Shared {
   double tab[64];
   u64 red[kThreads / 32];
-  u64 top[kMaxCluster], whole[kMaxCluster], above[kMaxCluster];
-  uint32_t least[kMaxCluster];
+  u64 whole[kMaxCluster], above[kMaxCluster];
+  float high[kMaxCluster], low[kMaxCluster], warp_high[kThreads / 32], warp_low[kThreads / 32];
   int listed;        // tokens gathered here
   int total;         // the row's list (first CTA)
   int place;         // where this CTA's part of it goes
@@ -193,7 +195,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   const int r = blockIdx.x / ctas, j0 = rank * p.slice, n = max(0, min(p.slice, a.vocab - j0));
   cluster.barrier_arrive();  // every CTA runs before any writes to another
   if (tid < 64) sh.tab[tid] = exp2(-tid / 64.0);
-  if (tid == 0) sh.listed = sh.total = 0;
+  if (tid == 0) {
+    sh.listed = sh.total = 0;
+    sh.pick_item = INT_MAX;
+  }
   serve_wait();
   serve_dependents();
   const T *row = static_cast<const T *>(a.logits) + r * a.stride + j0;
@@ -230,70 +235,76 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     for (int j = n + tid; j < (n + kVec - 1) / kVec * kVec; j += kThreads) slice[j] = from_f32<T>(-INFINITY);
     __syncthreads();
   }
-  u64 best = 0;            // the largest ord (0: none)
-  uint32_t least = ~0u;    // the least key
-  each([&](float l, int j) {
-    const uint32_t k = order_key(l);
-    const u64 o = token_ord(k, j);
-    best = k && o > best ? o : best;
-    least = k ? min(least, k) : least;
+  float high = -INFINITY, low = INFINITY;  // fmaxf and fminf pass over NaN
+  each([&](float l, int) {
+    high = fmaxf(high, l);
+    low = fminf(low, l);
   });
   const int group_threads = max(1, ctas * kThreads / kGroups), cta_groups = kThreads / group_threads;
   {
-    uint32_t g = static_cast<uint32_t>(best >> kIndexBits);
-    for (int o = 1; o < group_threads; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-    u64 b = best;
-    uint32_t lo = least;
+    float g = high;
+    for (int o = 1; o < group_threads; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    float hi = high, lo = low;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const u64 u = __shfl_xor_sync(0xffffffffu, b, o);
-      b = u > b ? u : b;
-      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     }
     if (lane == 0) {
-      sh.red[warp] = b;
-      sh.digits[warp] = lo;
+      sh.warp_high[warp] = hi;
+      sh.warp_low[warp] = lo;
     }
     __syncthreads();
     cluster.barrier_wait();
     if (top_k && !greedy && tid % group_threads == 0)
       for (int c = 0; c < ctas; ++c)
-        cluster.map_shared_rank(groups, c)[rank * cta_groups + tid / group_threads] = g;
+        cluster.map_shared_rank(groups, c)[rank * cta_groups + tid / group_threads] = order_key(g);
     if (tid < ctas) {
-      u64 m = 0;
-      uint32_t lw = ~0u;
       for (int w = 0; w < kThreads / 32; ++w) {
-        m = sh.red[w] > m ? sh.red[w] : m;
-        lw = min(lw, sh.digits[w]);
+        hi = fmaxf(hi, sh.warp_high[w]);
+        lo = fminf(lo, sh.warp_low[w]);
       }
       Shared *to = cluster.map_shared_rank(&sh, tid);
-      to->top[rank] = m;
-      to->least[rank] = lw;
+      to->high[rank] = hi;
+      to->low[rank] = lo;
     }
   }
   cluster.sync();
-  u64 top = 0;
-  uint32_t low = ~0u;
   for (int c = 0; c < ctas; ++c) {
-    top = sh.top[c] > top ? sh.top[c] : top;
-    low = min(low, sh.least[c]);
+    high = fmaxf(high, sh.high[c]);
+    low = fminf(low, sh.low[c]);
   }
-  if (top == 0 || greedy) {
+  if (high == -INFINITY) {  // nothing can be drawn
     if (rank == 0 && tid == 0) {
-      a.ids[r] = top == 0 ? -1 : (1 << kIndexBits) - 1 - static_cast<int>(top & ((1 << kIndexBits) - 1));
-      if (a.logprobs) a.logprobs[r] = top == 0 ? -INFINITY : 0.0f;
+      a.ids[r] = -1;
+      if (a.logprobs) a.logprobs[r] = -INFINITY;
     }
     return;
   }
+  if (greedy) {  // the first of the largest
+    int at = INT_MAX;
+    each([&](float l, int j) {
+      if (l == high) at = min(at, j);
+    });
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0 && at != INT_MAX) atomicMin(&first->pick_item, at);
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      a.ids[r] = sh.pick_item;
+      if (a.logprobs) a.logprobs[r] = 0.0f;
+    }
+    return;
+  }
+  const u64 top = token_ord(order_key(high), 0);  // no token's ord is larger
   RowRule rule;
-  rule.mx = key_logit(static_cast<uint32_t>(top >> kIndexBits));
-  rule.mxd = static_cast<double>(rule.mx);
+  rule.mx = high;
+  rule.mxd = static_cast<double>(high);
   rule.step = 64.0 * 1.4426950408889634 / static_cast<double>(temp);
   rule.scale = p.scale;
   rule.tab = sh.tab;
   {
     // steps over what the row spans, or down to weights that round to nothing
-    const float span = fminf(rule.mx - key_logit(low), 36.0f * temp);
+    const float span = fminf(high - low, 36.0f * temp);
     rule.bin_scale = span > 0.0f && span < INFINITY ? kBins / span : 0.0f;
   }
 
@@ -336,23 +347,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     // l >= max + T ln(min_p), a little lower: the list is cut exactly
     const double at = rule.mxd + static_cast<double>(temp) * log(static_cast<double>(min_p)) * (1.0 + 1e-6);
     const uint32_t k = order_key(__double2float_rd(at - 1e-6 * fabs(rule.mxd)));
-    bound = max(bound, min(k, static_cast<uint32_t>(top >> kIndexBits)));
+    bound = max(bound, min(k, order_key(high)));
     bounded = true;
   }
   __syncthreads();  // the groups have been read
 
   // ---- 2. the tokens that reach the bound
+  // (at most a few thousand tokens of a row are wanted: one atomic each)
   auto gather = [&](auto wanted) {  // into `gathered`, then to the first CTA's list
     each([&](float l, int j) {
-      const uint32_t k = order_key(l);
-      const bool want = k && wanted(l, k, j);
-      const unsigned bal = __ballot_sync(__activemask(), want);
-      if (want) {
-        const int lead = __ffs(bal) - 1;
-        int at = 0;
-        if (lane == lead) at = atomicAdd(&sh.listed, __popc(bal));
-        at = __shfl_sync(bal, at, lead) + __popc(bal & ((1u << lane) - 1u));
-        if (at < kListCap) gathered[at] = token_ord(k, j);
+      if (wanted(l, j)) {
+        const int at = atomicAdd(&sh.listed, 1);
+        if (at < kListCap) gathered[at] = token_ord(order_key(l), j);
       }
     });
     __syncthreads();
@@ -367,14 +373,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   const double min_share = ldexp(static_cast<double>(min_p), p.scale);
   u64 whole = 0, above = 0;
   if (bounded) {
-    gather([&](float, uint32_t k, int) { return k >= bound; });
+    const float least = bound > kKeyNegInf ? key_logit(bound) : -FLT_MAX;
+    gather([&](float l, int) { return l >= least; });
     if (top_p > 0.0f) each([&](float l, int) { whole += l > -INFINITY ? rule.weight(l) : 0; });
   } else {
     for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
     __syncthreads();
   }
   auto count_in = [&](uint32_t w_lo, uint32_t w_hi, int b) {
-    atomicAdd(&bin_count[b], 1u);
+    if (top_k) atomicAdd(&bin_count[b], 1u);
     const uint32_t old = atomicAdd(&bin_lo[b], w_lo);
     w_hi += old + w_lo < old ? 1u : 0u;
     if (w_hi) atomicAdd(&bin_hi[b], w_hi);
@@ -384,8 +391,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       if (!(l > -INFINITY)) return;
       const double s = rule.share(l);
       const u64 w = RowRule::round(s);
-      whole += w;
-      above += s >= min_share ? w : 0;
+      if (min_p > 0.0f) above += s >= min_share ? w : 0;
       count_in(static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32), rule.bin(l));
     });
   };
@@ -408,40 +414,28 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       c0[b] = cnt;
     }
   };
-  auto publish = [&]() {
-    whole = block_sum(whole, sh.red);
-    above = block_sum(above, sh.red);
-    if (tid == 0) {
-      first->whole[rank] = whole;
-      first->above[rank] = above;
-    }
+  auto publish = [&](u64 v, u64 (Shared::*to)[kMaxCluster]) {
+    v = block_sum(v, sh.red);
+    if (tid == 0) (first->*to)[rank] = v;
   };
-  bool have_hist = false;
-  if (!bounded) {
-    histogram();
-    publish();
-    collect(tot_mass, tot_count);
-    have_hist = true;
-  } else if (top_p > 0.0f) {
-    publish();
-  }
-  cluster.sync();
+  bool have_hist = !bounded;
   if (bounded) {
-    const bool overflow = first->total > kListCap;
-    cluster.barrier_arrive();  // the first CTA outlives the others' look at its memory
-    if (overflow) {  // too many reach the bound: by the histogram after all
+    if (top_p > 0.0f) publish(whole, &Shared::whole);
+    cluster.sync();
+    have_hist = first->total > kListCap;  // too many reach the bound: by the histogram after all
+    cluster.barrier_arrive();             // the first CTA outlives the others' look at its memory
+    if (!have_hist && rank != 0) return;
+    if (have_hist) {
       cluster.barrier_wait();
-      whole = above = 0;
       for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
       __syncthreads();
-      histogram();
-      publish();
-      collect(tot_mass, tot_count);
-      have_hist = true;
-      cluster.sync();
-    } else if (rank != 0) {
-      return;
     }
+  }
+  if (have_hist) {
+    histogram();
+    if (min_p > 0.0f) publish(above, &Shared::above);
+    collect(tot_mass, tot_count);
+    cluster.sync();
   }
 
   // ---- the first CTA decides, the others gather and divide as it says
@@ -565,10 +559,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   }
 
   // the tokens of a command's steps and range
-  auto in_command = [&](const Command &c, float l, uint32_t k, int j) {
-    const u64 o = token_ord(k, j);
+  auto in_command = [&](const Command &c, float l, int j) {
     const int b = rule.bin(l);
-    return b >= c.bin0 && b <= c.bin1 && o >= c.lo && o <= c.hi;
+    if (b < c.bin0 || b > c.bin1 || !(l > -INFINITY)) return false;
+    const u64 o = token_ord(order_key(l), j);
+    return o >= c.lo && o <= c.hi;
   };
   auto obey = [&]() -> bool {  // every CTA: false when the row is done
     cluster.sync();  // the command stands, the list is empty
@@ -578,14 +573,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       return false;
     }
     if (c.op == kGather) {
-      gather([&](float l, uint32_t k, int j) { return in_command(c, l, k, j); });
+      gather([&](float l, int j) { return in_command(c, l, j); });
     } else {
       for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
       __syncthreads();
       each([&](float l, int j) {
-        const uint32_t k = order_key(l);
-        if (!k || !in_command(c, l, k, j)) return;
-        const u64 w = rule.weight(l), s = (c.hi - token_ord(k, j)) >> c.shift;
+        if (!in_command(c, l, j)) return;
+        const u64 w = rule.weight(l), s = (c.hi - token_ord(order_key(l), j)) >> c.shift;
         count_in(static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32), static_cast<int>(min(s, (u64)(kBins - 1))));
       });
       collect(list, reinterpret_cast<uint32_t *>(list + kBins));
@@ -637,23 +631,34 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     c.hi = ~0ull;
     u64 before = sh.pick_before, before_n = sh.pick_before_count;
     int here = sh.pick_count;
-    *from_start = before_n + here <= kListCap;
+    *from_start = top_k && before_n + here <= kListCap;
     if (*from_start) {
       c.bin0 = 0;
       before = before_n = 0;
       here = 0;
     }
     __syncthreads();
-    // Divide the step by ord until it fits.  ord has 52 bits and each division takes
-    // 10 of them, after a first one by a range estimated from the step's logits (its
-    // last part takes what lies below the estimate): 7 suffice.
-    for (int level = 0; here > kListCap && level < 8; ++level) {
+    // List the step's tokens, or divide it by ord until they fit (the counts, kept for a
+    // top_k only, save an attempt).  ord has 52 bits and each division takes 10 of
+    // them, after a first one by a range estimated from the step's logits (its last
+    // part takes what lies below the estimate): 7 suffice.
+    for (int level = 0; level < 9; ++level) {
+      if (here <= kListCap) {
+        c.op = kGather;
+        if (tid == 0) {
+          sh.cmd = c;
+          sh.total = 0;
+        }
+        __syncthreads();
+        obey();
+        if (sh.total <= kListCap) break;
+      }
       if (level == 0) {
         const float w = rule.bin_scale > 0.0f ? 1.0f / rule.bin_scale : INFINITY;
-        const uint32_t kh = order_key(rule.mx - w * (static_cast<float>(c.bin0) - 0.5f));  // half a step over it
-        const uint32_t kl = order_key(rule.mx - w * static_cast<float>(c.bin0 + 1));
+        const uint32_t kh = order_key(high - w * (static_cast<float>(c.bin0) - 0.5f));  // half a step over it
+        const uint32_t kl = order_key(high - w * static_cast<float>(c.bin0 + 1)), k0 = order_key(low);
         c.hi = c.bin0 == 0 || kh == 0 ? top : token_ord(kh, 0);
-        const u64 lo = c.bin0 + 1 == kBins || kl < low ? static_cast<u64>(low) << kIndexBits : token_ord(kl, (1 << kIndexBits) - 1);
+        const u64 lo = c.bin0 + 1 == kBins || kl < k0 ? static_cast<u64>(k0) << kIndexBits : token_ord(kl, (1 << kIndexBits) - 1);
         c.shift = 0;
         while (c.hi > lo && ((c.hi - lo) >> c.shift) >= kBins) ++c.shift;
       }
@@ -667,21 +672,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       before_n = sh.pick_before_count;
       here = sh.pick_count;
       __syncthreads();
-      const u64 hi = c.hi - (s << c.shift);
-      if (s + 1 < kBins) c.lo = hi - ((1ull << c.shift) - 1);
-      c.hi = hi;
-      // the last step runs down to lo
+      c.hi -= s << c.shift;
+      if (s + 1 < kBins) c.lo = c.hi - ((1ull << c.shift) - 1);  // the last step runs down to lo
       const u64 size = c.hi - c.lo;
       c.shift = 0;
       while ((size >> c.shift) >= kBins) ++c.shift;
     }
-    c.op = kGather;
-    if (tid == 0) {
-      sh.cmd = c;
-      sh.total = 0;
-    }
-    __syncthreads();
-    obey();
     m = min(sh.total, kListCap);
     sort_list(m);
     list_sums(m, before, sums);
@@ -698,12 +694,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     return reach(m, sums, target, sum_there);
   };
   u64 z = 0, kept = 0, tokens = 0;
-  for (int c = 0; c < ctas; ++c) {
-    z += sh.whole[c];
-    kept += sh.above[c];
+  for (int b = tid; b < kBins; b += kThreads) {
+    z += tot_mass[b];
+    tokens += tot_count[b];
   }
-  for (int b = tid; b < kBins; b += kThreads) tokens += tot_count[b];
-  tokens = block_sum(tokens, sh.red);
+  z = block_sum(z, sh.red);
+  tokens = top_k ? block_sum(tokens, sh.red) : 0;
+  if (min_p > 0.0f)
+    for (int c = 0; c < ctas; ++c) kept += sh.above[c];
+  else
+    kept = z;
   bool from_start = false;
   u64 there;
   if (top_k && static_cast<u64>(top_k) < tokens) {
