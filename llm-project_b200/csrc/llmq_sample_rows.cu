@@ -56,43 +56,53 @@ __device__ __forceinline__ u64 token_ord(uint32_t key, int j) {
   return (static_cast<u64>(key) << kIndexBits) | static_cast<u64>((1 << kIndexBits) - 1 - j);
 }
 
-// exp on the way to an integer: 2^(-y / 64) for y = (max - l) * 64 log2(e) / T as
-// 2^-(n / 64) from a table, 2^-(n % 64 / 64), times the Taylor polynomial of
-// exp(-x), x = (y - n) ln 2 / 64, |x| < 0.0055, up to x^5 (the rest: 2^-54).
+// exp on the way to an integer: 2^(-y / 256) for y = (max - l) * 256 log2(e) / T as
+// 2^-(n / 256), n the integer next to y, from a table of 2^-(i / 256), times the
+// Taylor polynomial of 2^(-x / 256), |x| = |y - n| <= 1/2, up to x^4 (the rest: 2^-54).
+constexpr int kExpTable = 256;
 struct RowRule {
   float mx;            // the largest logit
-  double mxd, step;    // step: 64 log2(e) / T
+  bool infinite;       // it is +infinity: only its equals count, whatever T
+  double mxd, step;    // step: 256 log2(e) / T
   int scale;           // S
-  const double *tab;   // shared: 2^(-i / 64)
+  const double *tab;   // shared
   float bin_scale;     // steps of the histogram a unit of logit
 
-  // w * 2^S before rounding, for a token that is not excluded (0 beside an
-  // infinite maximum, whatever T)
+  // w * 2^S before rounding; 0 for NaN and -infinity
   __device__ __forceinline__ double share(float l) const {
-    const double y = (mxd - static_cast<double>(l)) * step;
-    if (!(y < 4032.0)) return l == mx ? __longlong_as_double(static_cast<long long>(1023 + scale) << 52) : 0.0;
+    if (infinite) return l == mx ? __hiloint2double((1023 + scale) << 20, 0) : 0.0;
+    const double y = (mxd - static_cast<double>(l)) * step;  // >= 0, or NaN
     const double yr = y + 6755399441055744.0;  // 1.5 * 2^52: the integer in the low bits
     const int n = __double2loint(yr);
-    const double x = (y - (yr - 6755399441055744.0)) * 0.010830424696249145;  // ln 2 / 64
-    double p = fma(x, -1.0 / 120.0, 1.0 / 24.0);
-    p = fma(x, p, -1.0 / 6.0);
-    p = fma(x, p, 0.5);
-    p = fma(x, p, -1.0);
+    const double x = y - (yr - 6755399441055744.0);
+    constexpr double c = -2.7076061740622863e-3;  // -ln 2 / 256
+    double p = fma(x, c * c * c * c / 24.0, c * c * c / 6.0);
+    p = fma(x, p, c * c / 2.0);
+    p = fma(x, p, c);
     p = fma(x, p, 1.0);
-    const double t = tab[n & 63];
-    return p * __hiloint2double(__double2hiint(t) + ((scale - (n >> 6)) << 20), __double2loint(t));
+    const double t = tab[n & (kExpTable - 1)];
+    const double s = p * __hiloint2double(__double2hiint(t) + ((scale - (n >> 8)) << 20), __double2loint(t));
+    return static_cast<uint32_t>(__double2hiint(y)) < 0x40cf8000u ? s : 0.0;  // y < 16128 (2^-63), no NaN of either sign
   }
   static __device__ __forceinline__ u64 round(double s) {
     const double r = s + 6755399441055744.0;  // s < 2^51
     return static_cast<u64>(__double_as_longlong(r)) - 0x4338000000000000ull;
   }
   __device__ __forceinline__ u64 weight(float l) const { return round(share(l)); }
-  // the histogram's step: any function that does not fall as l falls will do
+  // the histogram's step: any function that does not fall as l falls will do (the
+  // integer next to the product; NaN goes last)
   __device__ __forceinline__ int bin(float l) const {
-    const float d = mx - l;
-    if (l == mx) return 0;
-    const float x = d * bin_scale;
-    return x < kBins - 1 ? static_cast<int>(x) : kBins - 1;
+    const float x = fminf((mx - l) * bin_scale, static_cast<float>(kBins - 1)) + 8388608.0f;
+    return __float_as_int(x) & (kBins - 1);
+  }
+  __device__ __forceinline__ void set(float high, float temp, int bits, const double *table) {
+    mx = __fadd_rn(high, 0.0f);  // +0, not -0: no difference below is -0
+    infinite = high == INFINITY;
+    mxd = static_cast<double>(mx);
+    step = kExpTable * 1.4426950408889634 / static_cast<double>(temp);
+    scale = bits;
+    tab = table;
+    bin_scale = 0.0f;
   }
 };
 
@@ -106,7 +116,7 @@ enum { kDone = 0, kGather = 1, kDivide = 2 };
 
 // What each CTA keeps in static shared memory; the first CTA's is the row's.
 struct Shared {
-  double tab[64];
+  double tab[kExpTable];
   u64 red[kThreads / 32];
   u64 whole[kMaxCluster], above[kMaxCluster];
   float high[kMaxCluster], low[kMaxCluster], warp_high[kThreads / 32], warp_low[kThreads / 32];
@@ -130,13 +140,14 @@ __device__ __forceinline__ u64 warp_scan(u64 v) {
   return v;
 }
 // Inclusive sum over the block's threads; every thread of the block calls this.
+template <int NT = kThreads>
 __device__ __forceinline__ u64 block_scan(u64 v, u64 *red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v = warp_scan(v);
   __syncthreads();
   if (lane == 31) red[warp] = v;
   __syncthreads();
-  const u64 w = warp_scan(lane < kThreads / 32 ? red[lane] : 0);
+  const u64 w = warp_scan(lane < NT / 32 ? red[lane] : 0);
   const u64 before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
   return warp ? v + before : v;
 }
@@ -194,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x / ctas, j0 = rank * p.slice, n = max(0, min(p.slice, a.vocab - j0));
   cluster.barrier_arrive();  // every CTA runs before any writes to another
-  if (tid < 64) sh.tab[tid] = exp2(-tid / 64.0);
+  if (tid < kExpTable) sh.tab[tid] = exp2(-tid / static_cast<double>(kExpTable));
   if (tid == 0) {
     sh.listed = sh.total = 0;
     sh.pick_item = INT_MAX;
@@ -208,16 +219,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   const float top_p = a.top_p && a.top_p[r] > 0.0f && a.top_p[r] < 1.0f ? a.top_p[r] : 0.0f;
   const int top_k = a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.vocab ? a.top_k[r] : 0;
 
-  // f(logit, index) for every token of the slice
+  // f(logit, index) for every token of the slice, the next vector on its way meanwhile
+  const T *src = p.resident ? slice : row;
+  const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));
+  const int nv = (n - head) / kVec;
   auto each = [&](auto f) {
-    if (p.resident) {
-      for (int v = tid; v < (n + kVec - 1) / kVec; v += kThreads) {
-        const Pack<T, kVec> x = reinterpret_cast<const Pack<T, kVec> *>(slice)[v];
+    const Pack<T, kVec> *vec = reinterpret_cast<const Pack<T, kVec> *>(src + head);
+    Pack<T, kVec> next;
+    if (tid < nv) next = vec[tid];
+    for (int v = tid; v < nv; v += kThreads) {
+      const Pack<T, kVec> x = next;
+      if (v + kThreads < nv) next = vec[v + kThreads];
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) f(to_f32(x.v[i]), j0 + v * kVec + i);
-      }
-    } else {
-      for (int j = tid; j < n; j += kThreads) f(to_f32(row[j]), j0 + j);
+      for (int i = 0; i < kVec; ++i) f(to_f32(x.v[i]), j0 + head + v * kVec + i);
+    }
+#pragma unroll 1
+    for (int e = tid; e < n - kVec * nv; e += kThreads) {
+      const int j = e < head ? e : e + kVec * nv;
+      f(to_f32(src[j]), j0 + j);
     }
   };
 
@@ -232,7 +251,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
 #pragma unroll 4
       for (int j = tid; j < n; j += kThreads) slice[j] = row[j];
     }
-    for (int j = n + tid; j < (n + kVec - 1) / kVec * kVec; j += kThreads) slice[j] = from_f32<T>(-INFINITY);
     __syncthreads();
   }
   float high = -INFINITY, low = INFINITY;  // fmaxf and fminf pass over NaN
@@ -297,15 +315,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   }
   const u64 top = token_ord(order_key(high), 0);  // no token's ord is larger
   RowRule rule;
-  rule.mx = high;
-  rule.mxd = static_cast<double>(high);
-  rule.step = 64.0 * 1.4426950408889634 / static_cast<double>(temp);
-  rule.scale = p.scale;
-  rule.tab = sh.tab;
+  rule.set(high, temp, p.scale, sh.tab);
   {
     // steps over what the row spans, or down to weights that round to nothing
     const float span = fminf(high - low, 36.0f * temp);
-    rule.bin_scale = span > 0.0f && span < INFINITY ? kBins / span : 0.0f;
+    if (span > 0.0f && span < INFINITY) rule.bin_scale = fminf(kBins / span, 1e30f);
   }
 
   // ---- a bound that the tokens of every cut reach
@@ -375,24 +389,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   if (bounded) {
     const float least = bound > kKeyNegInf ? key_logit(bound) : -FLT_MAX;
     gather([&](float l, int) { return l >= least; });
-    if (top_p > 0.0f) each([&](float l, int) { whole += l > -INFINITY ? rule.weight(l) : 0; });
+    if (top_p > 0.0f) each([&](float l, int) { whole += rule.weight(l); });
   } else {
     for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
     __syncthreads();
   }
-  auto count_in = [&](uint32_t w_lo, uint32_t w_hi, int b) {
+  auto count_in = [&](u64 w, int b) {
+    if (w == 0) return;  // nothing to any sum
+    const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&bin_lo[b], lo);
+    const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old ? 1u : 0u);
+    if (hi) atomicAdd(&bin_hi[b], hi);
     if (top_k) atomicAdd(&bin_count[b], 1u);
-    const uint32_t old = atomicAdd(&bin_lo[b], w_lo);
-    w_hi += old + w_lo < old ? 1u : 0u;
-    if (w_hi) atomicAdd(&bin_hi[b], w_hi);
   };
   auto histogram = [&]() {
     each([&](float l, int) {
-      if (!(l > -INFINITY)) return;
       const double s = rule.share(l);
       const u64 w = RowRule::round(s);
       if (min_p > 0.0f) above += s >= min_share ? w : 0;
-      count_in(static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32), rule.bin(l));
+      count_in(w, rule.bin(l));
     });
   };
   // the row's histogram in the first CTA, each CTA summing a part of the steps
@@ -580,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       each([&](float l, int j) {
         if (!in_command(c, l, j)) return;
         const u64 w = rule.weight(l), s = (c.hi - token_ord(order_key(l), j)) >> c.shift;
-        count_in(static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32), static_cast<int>(min(s, (u64)(kBins - 1))));
+        count_in(w, static_cast<int>(min(s, (u64)(kBins - 1))));
       });
       collect(list, reinterpret_cast<uint32_t *>(list + kBins));
     }
@@ -653,9 +667,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
         obey();
         if (sh.total <= kListCap) break;
       }
+      *from_start = false;  // tokens of no weight, which are not counted, did not fit
       if (level == 0) {
         const float w = rule.bin_scale > 0.0f ? 1.0f / rule.bin_scale : INFINITY;
-        const uint32_t kh = order_key(high - w * (static_cast<float>(c.bin0) - 0.5f));  // half a step over it
+        const uint32_t kh = order_key(high - w * static_cast<float>(c.bin0 - 1));  // over the step
         const uint32_t kl = order_key(high - w * static_cast<float>(c.bin0 + 1)), k0 = order_key(low);
         c.hi = c.bin0 == 0 || kh == 0 ? top : token_ord(kh, 0);
         const u64 lo = c.bin0 + 1 == kBins || kl < k0 ? static_cast<u64>(k0) << kIndexBits : token_ord(kl, (1 << kIndexBits) - 1);
@@ -733,27 +748,512 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   obey();
 }
 
-template <typename T>
-cudaError_t launch(const LlmqSampleRows &a, int sms, cudaStream_t st) {
-  RowArgs p{};
-  p.a = a;
+
+// ------------------------------------------------------------- bf16 rows
+// A bf16 row has few distinct values, so a histogram of the values themselves needs
+// one 32-bit count a token and no exponential: the sum of w of a value is its
+// count times its w.  The cuts and the draw find their value by prefix sums, and
+// a tie is settled by counting in index order: no list, no sort.
+//
+// The histogram spans the 2048 magnitudes (16 binades) below the larger of |max l|
+// and |max(min l, max l - 36 T)| for either sign; what is lower has weights that
+// round to nothing.  Zero has a place of its own; the few logits nearer to it than the
+// span's least (2^-16 of the largest) share one place a sign, their sums formed
+// token by token, and a cut or draw that falls there is found by a slow search
+// (rows of nothing but such logits aside, about one in 10^4).  An f16 row has
+// eight times the values: it goes with the f32 ones.
+constexpr int kVals = 2048;
+// places, in falling order of their logits
+constexpr int kTinyPos = kVals, kZeroAt = kVals + 1, kTinyNeg = kVals + 2, kNeg0 = kVals + 3;
+constexpr int kPlaces = 2 * kVals + 3;
+constexpr int kValueThreads = 512;
+constexpr int kAhead = 3;  // vectors of 16 bytes a thread has in flight while it counts as many
+
+// Where a place is counted: positive magnitudes upwards, then negative ones upwards
+// and the three about zero, so that a token's index is its bits and one product away.
+__device__ __forceinline__ int count_index(int place) {
+  return place < kVals ? kVals - 1 - place : place >= kNeg0 ? kVals + place - kNeg0 : 2 * kVals + place - kTinyPos;
+}
+
+struct ValueShared {
+  double tab[kExpTable];
+  u64 red[kValueThreads / 32];
+  float warp_high[kValueThreads / 32], warp_low[kValueThreads / 32];
+  // written by every CTA of the row into every other
+  float high[kMaxCluster], low[kMaxCluster];
+  u64 mass[kMaxCluster], count[kMaxCluster], above[kMaxCluster];
+  // of this CTA: the places that counters keep (kTinyPos, kZeroAt, kTinyNeg)
+  u64 tiny_mass[3], tiny_above[3];
+  // what the owner of a cut's place tells (top_k's, top_p's, the draw's)
+  struct {
+    int place;
+    u64 before, before_n;
+  } told[3];
+  u64 bins[256];
+  u64 pick[2];
+};
+
+template <int NT>
+__device__ __forceinline__ u64 block_sum_n(u64 v, u64 *red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) v += red[w];
+  return v;
+}
+
+__device__ __forceinline__ float bf16_bits(uint32_t b) { return __uint_as_float(b << 16); }
+
+// Logits before the first on 16 bytes.
+__device__ __forceinline__ int to_vector(const unsigned short *row) {
+  return static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / 2);
+}
+
+__global__ void __launch_bounds__(kValueThreads, 2) k_sample_values(const RowArgs p) {
+  extern __shared__ __align__(16) unsigned char s_dyn[];
+  __shared__ ValueShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int own = (kPlaces + ctas - 1) / ctas, p0 = rank * own, p1 = min(kPlaces, p0 + own);  // the places this CTA sums
+  uint32_t *count = reinterpret_cast<uint32_t *>(s_dyn);  // [kPlaces], of this CTA's tokens
+  u64 *mass = reinterpret_cast<u64 *>(count + (kPlaces + 3) / 4 * 4);  // [own], of the row
+  uint32_t *total = reinterpret_cast<uint32_t *>(mass + own);          // [own], of the row
+  const LlmqSampleRows &a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = blockIdx.x / ctas, j0 = rank * p.slice, n = max(0, min(p.slice, a.vocab - j0));
+  cluster.barrier_arrive();
+  if (tid < kExpTable) sh.tab[tid] = exp2(-tid / static_cast<double>(kExpTable));
+  if (tid < 3) sh.tiny_mass[tid] = sh.tiny_above[tid] = 0;
+  for (int i = tid; i < kPlaces; i += kValueThreads) count[i] = 0;
+  serve_wait();
+  serve_dependents();
+  const unsigned short *whole_row = static_cast<const unsigned short *>(a.logits) + r * a.stride, *row = whole_row + j0;
+  const float temp = a.temperature ? a.temperature[r] : 1.0f;
+  const bool greedy = !(temp > 0.0f);
+  const float min_p = a.min_p && a.min_p[r] > 0.0f ? fminf(a.min_p[r], 1.0f) : 0.0f;
+  const float top_p = a.top_p && a.top_p[r] > 0.0f && a.top_p[r] < 1.0f ? a.top_p[r] : 0.0f;
+  const int top_k = a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.vocab ? a.top_k[r] : 0;
+
+  // ---- the largest and least logit (of two at a time; NaN is passed over)
+  float high = -INFINITY, low = INFINITY;
+  {
+    const __nv_bfloat162 nan = __floats2bfloat162_rn(NAN, NAN);
+    __nv_bfloat162 hi2 = nan, lo2 = nan;
+    const int head = min(n, to_vector(row)), nv = (n - head) / 8;
+    const uint4 *vec = reinterpret_cast<const uint4 *>(row + head);
+    auto add2 = [&](uint32_t w) {
+      const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&w);
+      hi2 = __hmax2(hi2, x);
+      lo2 = __hmin2(lo2, x);
+    };
+    for (int v = tid; v < nv; v += 8 * kValueThreads) {
+      uint4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = v + i * kValueThreads < nv ? vec[v + i * kValueThreads] : make_uint4(~0u, ~0u, ~0u, ~0u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        add2(x[i].x);
+        add2(x[i].y);
+        add2(x[i].z);
+        add2(x[i].w);
+      }
+    }
+    for (int e = tid; e < n - 8 * nv; e += kValueThreads) {  // the ends
+      const float l = bf16_bits(row[e < head ? e : e + 8 * nv]);
+      high = fmaxf(high, l);
+      low = fminf(low, l);
+    }
+    high = fmaxf(high, fmaxf(__low2float(hi2), __high2float(hi2)));
+    low = fminf(low, fminf(__low2float(lo2), __high2float(lo2)));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+  }
+  if (lane == 0) {
+    sh.warp_high[warp] = high;
+    sh.warp_low[warp] = low;
+  }
+  __syncthreads();
+  cluster.barrier_wait();
+  if (tid < ctas) {
+    for (int w = 0; w < kValueThreads / 32; ++w) {
+      high = fmaxf(high, sh.warp_high[w]);
+      low = fminf(low, sh.warp_low[w]);
+    }
+    ValueShared *to = cluster.map_shared_rank(&sh, tid);
+    to->high[rank] = high;
+    to->low[rank] = low;
+  }
+  cluster.sync();
+  for (int c = 0; c < ctas; ++c) {
+    high = fmaxf(high, sh.high[c]);
+    low = fminf(low, sh.low[c]);
+  }
+  if (high == -INFINITY) {  // nothing can be drawn
+    if (rank == 0 && tid == 0) {
+      a.ids[r] = -1;
+      if (a.logprobs) a.logprobs[r] = -INFINITY;
+    }
+    return;
+  }
+  RowRule rule;
+  rule.set(high, temp, p.scale, sh.tab);
+  const double min_share = ldexp(static_cast<double>(min_p), p.scale);
+  // the span's least magnitude
+  const float far = fmaxf(fabsf(high), greedy ? 0.0f : fabsf(fmaxf(low, high - 36.0f * temp)));
+  const int least = min(max(static_cast<int>(__float_as_uint(far) >> 16) + 1 - kVals, 1), 0x7f81 - kVals);
+  auto value_at = [&](int place) -> float {  // a place of one value
+    if (place < kVals) return bf16_bits(least + kVals - 1 - place);
+    return place >= kNeg0 ? bf16_bits((least + place - kNeg0) | 0x8000u) : 0.0f;
+  };
+  auto one_value = [&](int place) { return place != kTinyPos && place != kTinyNeg; };
+  int place = 0;
+  u64 nth = 1, kept = 0;
+  if (greedy) {
+    place = high == 0.0f ? kZeroAt : high > 0.0f ? kVals - 1 + least - static_cast<int>(__float_as_uint(high) >> 16)
+                                                 : kNeg0 + static_cast<int>((__float_as_uint(high) >> 16) & 0x7fffu) - least;
+  }
+
+  // ---- counts of values, without a branch: the byte offset of a token's count is
+  // 4 (magnitude - least) + (negative ? 4 kVals : 0), and 4 kVals is its sign bit / 4
+  static_assert(4 * kVals == 0x8000 / 4, "the sign bit moves to its offset");
+  const uint32_t counts = static_cast<uint32_t>(__cvta_generic_to_shared(count));
+  uint32_t zeros = 0, pos_n = 0, neg_n = 0;
+  u64 pos_m = 0, neg_m = 0, pos_a = 0, neg_a = 0;
+  auto add = [&](uint32_t mag, uint32_t sign) -> int {  // sign: in bit 15
+    const int x = static_cast<int>(mag) - least;
+    // what lies past the span is too low to count, -infinity or NaN
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.lt.u32 q, %0, %1;\n\t@q red.shared.add.u32 [%2], 1;\n\t}" ::"r"(x), "n"(kVals),
+        "r"(counts + 4 * x + ((sign >> 2) & 0x2000u))
+        : "memory");
+    return x;  // below 0: nearer to zero than the span
+  };
+  auto add2 = [&](uint32_t w) -> int {
+    const uint32_t m = w & 0x7fff7fffu;
+    return add(m & 0xffffu, w) | add(m >> 16, w >> 16);
+  };
+  auto add_near = [&](uint32_t b) {
+    const int mag = b & 0x7fff;
+    if (mag >= least) return;
+    if (mag == 0) {
+      ++zeros;
+      return;
+    }
+    const double s = rule.share(bf16_bits(b));
+    const u64 w = RowRule::round(s), v = s >= min_share ? w : 0;
+    if (b & 0x8000u) {
+      ++neg_n;
+      neg_m += w;
+      neg_a += v;
+    } else {
+      ++pos_n;
+      pos_m += w;
+      pos_a += v;
+    }
+  };
+  {
+    const int head = min(n, to_vector(row)), nv = (n - head) / 8;
+    const uint4 *vec = reinterpret_cast<const uint4 *>(row + head);
+    uint4 x[kAhead], next[kAhead];
+    auto fetch = [&](int v) {  // what is past the end counts as NaN
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        next[i] = v + i * kValueThreads < nv ? vec[v + i * kValueThreads] : make_uint4(~0u, ~0u, ~0u, ~0u);
+    };
+    fetch(tid);
+    for (int v = tid; v < nv; v += kAhead * kValueThreads) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) x[i] = next[i];
+      fetch(v + kAhead * kValueThreads);
+      int near = 0;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) near |= add2(x[i].x) | add2(x[i].y) | add2(x[i].z) | add2(x[i].w);
+      if (near < 0) {  // seldom: read them again
+#pragma unroll 1
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll 1
+          for (int e = 0; e < 8 && v + i * kValueThreads < nv; ++e) add_near(row[head + 8 * (v + i * kValueThreads) + e]);
+      }
+    }
+#pragma unroll 1
+    for (int e = tid; e < n - 8 * nv; e += kValueThreads) {  // the ends
+      const uint32_t b = row[e < head ? e : e + 8 * nv];
+      if (add(b & 0x7fffu, b) < 0) add_near(b);
+    }
+  }
+  if (zeros) atomicAdd(&count[count_index(kZeroAt)], zeros);
+  if (pos_n) {
+    atomicAdd(&count[count_index(kTinyPos)], pos_n);
+    atomicAdd(&sh.tiny_mass[0], pos_m);
+    atomicAdd(&sh.tiny_above[0], pos_a);
+  }
+  if (neg_n) {
+    atomicAdd(&count[count_index(kTinyNeg)], neg_n);
+    atomicAdd(&sh.tiny_mass[2], neg_m);
+    atomicAdd(&sh.tiny_above[2], neg_a);
+  }
+  cluster.sync();
+
+  if (!greedy) {
+    // ---- each CTA sums its places over the cluster, a thread `per` adjacent ones (odd: no
+    // two lanes of a warp in one bank)
+    for (int i = p0 + tid; i < p1; i += kValueThreads) {
+      const int at = count_index(i);
+      uint32_t c = 0;
+      for (int q = 0; q < ctas; ++q) c += cluster.map_shared_rank(count, q)[at];
+      total[i - p0] = c;
+    }
+    __syncthreads();
+    const int per = ((own + kValueThreads - 1) / kValueThreads) | 1;
+    const int i0 = min(p1 - p0, tid * per), i1 = min(p1 - p0, i0 + per);
+    u64 mine_m = 0, mine_n = 0, mine_a = 0;
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t c = total[i];
+      u64 m = 0, v = 0;
+      if (c && one_value(p0 + i)) {
+        const double s = rule.share(value_at(p0 + i));
+        m = c * RowRule::round(s);
+        v = s >= min_share ? m : 0;
+      } else if (c) {
+        for (int q = 0; q < ctas; ++q) {
+          const ValueShared *o = cluster.map_shared_rank(&sh, q);
+          m += o->tiny_mass[p0 + i - kTinyPos];
+          v += o->tiny_above[p0 + i - kTinyPos];
+        }
+      }
+      mass[i] = m;
+      mine_m += m;
+      mine_n += c;
+      mine_a += v;
+    }
+    // sums and counts up to and with each thread's places
+    const u64 upto_m = block_scan<kValueThreads>(mine_m, sh.red);
+    const u64 upto_n = top_k ? block_scan<kValueThreads>(mine_n, sh.red) : 0;
+    if (min_p > 0.0f) mine_a = block_sum_n<kValueThreads>(mine_a, sh.red);
+    if (tid == kValueThreads - 1)
+      for (int q = 0; q < ctas; ++q) {
+        ValueShared *to = cluster.map_shared_rank(&sh, q);
+        to->mass[rank] = upto_m;
+        to->count[rank] = upto_n;
+        to->above[rank] = mine_a;
+      }
+    cluster.sync();
+    u64 z = 0, usable = 0, above = 0;
+    for (int c = 0; c < ctas; ++c) {
+      z += sh.mass[c];
+      usable += sh.count[c];
+      above += sh.above[c];
+    }
+    kept = min_p > 0.0f ? above : z;
+
+    // Every CTA: the place where the measure (counts or sums) reaches target, and both up
+    // to it.  The CTA that owns the place tells the others.
+    u64 before = 0, before_n = 0;
+    auto find = [&](int which, bool by_count, u64 target) {
+      u64 bm = 0, bn = 0;
+      int owner = 0;
+      for (; owner + 1 < ctas; ++owner) {
+        if ((by_count ? bn + sh.count[owner] : bm + sh.mass[owner]) >= target) break;
+        bm += sh.mass[owner];
+        bn += sh.count[owner];
+      }
+      if (owner == rank) {
+        u64 am = bm + upto_m - mine_m, ac = by_count ? bn + upto_n - mine_n : 0;
+        if ((by_count ? ac : am) < target && (by_count ? ac + mine_n : am + mine_m) >= target) {  // one thread
+          int i = i0;
+          for (; (by_count ? ac + total[i] : am + mass[i]) < target; ++i) {
+            am += mass[i];
+            ac += total[i];
+          }
+          for (int q = 0; q < ctas; ++q) {
+            auto *to = &cluster.map_shared_rank(&sh, q)->told[which];
+            to->place = p0 + i;
+            to->before = am;
+            to->before_n = ac;
+          }
+        }
+      }
+      cluster.sync();
+      place = sh.told[which].place;
+      before = sh.told[which].before;
+      before_n = sh.told[which].before_n;
+    };
+    // Within a place of many values, from `before` on: the key and what precedes it, by
+    // every CTA alone over the whole row (slow; see above)
+    uint32_t key = 0;
+    auto find_tiny = [&](bool by_count, u64 target) {
+      const bool neg = place == kTinyNeg;
+      uint32_t prefix = 0, mask = 0;
+      for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
+        for (int i = tid; i < 256; i += kValueThreads) sh.bins[i] = 0;
+        __syncthreads();
+        for (int j = tid; j < a.vocab; j += kValueThreads) {
+          const uint32_t b = whole_row[j];
+          const int mag = b & 0x7fff;
+          const uint32_t k = order_key(bf16_bits(b));
+          if (mag > 0 && mag < least && static_cast<bool>(b & 0x8000u) == neg && (k & mask) == prefix)
+            atomicAdd(&sh.bins[(k >> shift) & 255u], by_count ? 1ull : rule.weight(bf16_bits(b)));
+        }
+        __syncthreads();
+        if (tid == 0) {
+          u64 at = by_count ? before_n : before;
+          int d = 255;
+          for (; d > 0 && at + sh.bins[d] < target; --d) at += sh.bins[d];
+          sh.pick[0] = d;
+          sh.pick[1] = at;
+        }
+        __syncthreads();
+        (by_count ? before_n : before) = sh.pick[1];
+        prefix |= static_cast<uint32_t>(sh.pick[0]) << shift;
+        mask |= 255u << shift;
+      }
+      key = prefix;
+      if (by_count) {  // the sum of what precedes the key
+        u64 m = 0;
+        for (int j = tid; j < a.vocab; j += kValueThreads) {
+          const uint32_t b = whole_row[j];
+          const int mag = b & 0x7fff;
+          const float l = bf16_bits(b);
+          if (mag > 0 && mag < least && static_cast<bool>(b & 0x8000u) == neg && order_key(l) > key) m += rule.weight(l);
+        }
+        before += block_sum_n<kValueThreads>(m, sh.red);
+      }
+    };
+    auto reach = [&](int which, bool by_count, u64 target) -> u64 {  // its w
+      find(which, by_count, target);
+      if (!one_value(place)) {
+        find_tiny(by_count, target);
+        return rule.weight(key_logit(key));
+      }
+      return rule.weight(value_at(place));
+    };
+    if (top_k && static_cast<u64>(top_k) < usable) {
+      const u64 w = reach(0, true, top_k);
+      kept = min(kept, before + (top_k - before_n) * w);
+    }
+    if (top_p > 0.0f) {
+      const u64 target = part_of(top_p, z);
+      if (target < kept) {
+        const u64 w = reach(1, false, target);
+        kept = min(kept, before + (target - before + w - 1) / w * w);
+      }
+    }
+    const float uf = a.u[r];
+    const u64 target = part_of(uf > 0.0f ? fminf(uf, 1.0f) : 0.0f, kept);
+    const u64 w = reach(2, false, target);
+    nth = (target - before + w - 1) / w;
+    if (!one_value(place)) {  // among all tokens of the row with this key, by the first CTA alone
+      const uint32_t code = __float_as_uint(key_logit(key)) >> 16;
+      if (rank == 0 && warp == 0) {
+        u64 seen = 0;
+        for (int j1 = 0; j1 < a.vocab && seen < nth; j1 += 32) {
+          const unsigned bal = __ballot_sync(0xffffffffu, j1 + lane < a.vocab && whole_row[j1 + lane] == code);
+          if (((bal >> lane) & 1u) && seen + __popc(bal & ((1u << lane) - 1u)) + 1 == nth) {
+            a.ids[r] = j1 + lane;
+            if (a.logprobs) {
+              const double lw = -(rule.mxd - static_cast<double>(key_logit(key))) / static_cast<double>(temp);
+              a.logprobs[r] = static_cast<float>(lw - log(ldexp(static_cast<double>(kept), -p.scale)));
+            }
+          }
+          seen += __popc(bal);
+        }
+      }
+      return;
+    }
+  }
+
+  // ---- the nth token of the place's value, in index order
+  int owner = 0;
+  {
+    const uint32_t c = lane < ctas ? cluster.map_shared_rank(count, lane)[count_index(place)] : 0;
+    const u64 upto = warp_scan(c);
+    const unsigned who = __ballot_sync(0xffffffffu, lane < ctas && upto >= nth);
+    owner = __ffs(who) - 1;
+    nth -= __shfl_sync(0xffffffffu, upto - c, owner & 31);
+  }
+  cluster.barrier_arrive();  // a CTA outlives the others' look at its counts
+  if (owner == rank) {
+    // each warp a part of the slice, 16 bytes a lane and step (+0 and -0 compare as equal)
+    const float want = value_at(place);
+    const uint32_t code = __float_as_uint(want) >> 16, ignore = place == kZeroAt ? 0x7fffu : 0xffffu;
+    const int head = min(n, to_vector(row)), nv = (n - head) / 8, part = (nv + kValueThreads - 1) / kValueThreads * 32;
+    const int va = min(nv, warp * part), vb = min(nv, va + part);
+    const uint4 *vec = reinterpret_cast<const uint4 *>(row + head);
+    const uint32_t code2 = code | (code << 16);
+    auto hits = [&](uint32_t w) -> uint32_t {  // bit 0 and bit 16: the halves that match
+      return __heq2_mask(*reinterpret_cast<const __nv_bfloat162 *>(&w), *reinterpret_cast<const __nv_bfloat162 *>(&code2)) &
+             0x00010001u;
+    };
+    auto hits8 = [&](const uint4 x) { return hits(x.x) + hits(x.y) + hits(x.z) + hits(x.w); };
+    uint32_t c2 = 0;  // two counts of at most 2^15 / 32 steps of 4
+#pragma unroll 4
+    for (int v = va + lane; v < vb; v += 32) c2 += hits8(vec[v]);
+    int c = static_cast<int>((c2 & 0xffffu) + (c2 >> 16));
+    c = __reduce_add_sync(0xffffffffu, c);
+    // what does not fill a vector: the head before all, the tail behind all
+    auto single = [&](int j) { return (row[j] & ignore) == code; };
+    if (lane == 0) sh.red[warp] = c;
+    const unsigned head_bal = __ballot_sync(0xffffffffu, lane < head && single(lane));
+    __syncthreads();
+    u64 seen = __popc(head_bal);
+    auto tell = [&](int j) {
+      a.ids[r] = j0 + j;
+      if (a.logprobs) {
+        const double lw = want == high ? 0.0 : -(rule.mxd - static_cast<double>(want)) / static_cast<double>(temp);
+        a.logprobs[r] = greedy ? 0.0f : static_cast<float>(lw - log(ldexp(static_cast<double>(kept), -p.scale)));
+      }
+    };
+    if (nth <= seen) {  // in the head
+      if (warp == 0 && ((head_bal >> lane) & 1u) && __popc(head_bal & ((1u << lane) - 1u)) + 1 == nth) tell(lane);
+    } else {
+      for (int w = 0; w < warp; ++w) seen += sh.red[w];
+      if (seen < nth && seen + c >= nth) {
+        for (int v0 = va; v0 < vb && seen < nth; v0 += 32) {
+          const int v = v0 + lane;
+          const uint4 x = v < vb ? vec[v] : make_uint4(0, 0, 0, 0);
+          const uint32_t h = v < vb ? hits8(x) : 0u;
+          const int mine = static_cast<int>((h & 0xffffu) + (h >> 16));
+          const int incl = static_cast<int>(warp_scan(mine));
+          if (seen + incl >= nth && seen + incl - mine < nth) {
+            int left = static_cast<int>(nth - seen) - (incl - mine), j = head + 8 * v;
+            for (; left > 0; ++j) left -= single(j);
+            tell(j - 1);
+          }
+          seen += __shfl_sync(0xffffffffu, incl, 31);
+        }
+      }
+      if (warp == kValueThreads / 32 - 1 && seen + c < nth) {  // in the tail
+        const int j = head + 8 * nv + lane;
+        const unsigned bal = __ballot_sync(0xffffffffu, j < n && single(j));
+        if (((bal >> lane) & 1u) && seen + c + __popc(bal & ((1u << lane) - 1u)) + 1 == nth) tell(j);
+      }
+    }
+  }
+  cluster.barrier_wait();
+}
+
+inline int scale_bits(int vocab) {
   int log2v = 0;
-  while ((1 << log2v) < a.vocab) ++log2v;
-  p.scale = 62 - log2v < 50 ? 62 - log2v : 50;
-  // CTAs a row: a slice of at most 64 KB (two CTAs an SM), more while SMs idle
-  int ctas = 1;
-  auto slice_of = [&](int c) { return ((a.vocab + c - 1) / c + 15) / 16 * 16; };
-  while (ctas < kMaxCluster && (slice_of(ctas) * sizeof(T) > 64 * 1024 ||
-                                ((long long)a.n_rows * ctas < 2 * sms && slice_of(ctas) > 2 * kThreads)))
-    ctas *= 2;
-  p.slice = slice_of(ctas);
-  p.resident = p.slice * sizeof(T) <= 160 * 1024;
-  const int smem = kWorkBytes + (p.resident ? p.slice * (int)sizeof(T) : 0);
-  cudaError_t e = cudaFuncSetAttribute(k_sample_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  while ((1 << log2v) < vocab) ++log2v;
+  return 62 - log2v < 50 ? 62 - log2v : 50;
+}
+
+// A launch of n_rows clusters of `ctas` CTAs, with programmatic dependent launch.
+cudaError_t launch_clusters(void (*kern)(RowArgs), const RowArgs &p, int ctas, int threads, int smem, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.n_rows) * ctas);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(p.a.n_rows) * ctas);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2]{};
@@ -764,7 +1264,36 @@ cudaError_t launch(const LlmqSampleRows &a, int sms, cudaStream_t st) {
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, k_sample_rows<T>, p);
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+cudaError_t launch_values(const LlmqSampleRows &a, int sms, cudaStream_t st) {
+  RowArgs p{};
+  p.a = a;
+  p.scale = scale_bits(a.vocab);
+  int ctas = 1;
+  while (ctas < kMaxCluster && (long long)a.n_rows * ctas < sms && a.vocab / ctas > 4 * kValueThreads) ctas *= 2;
+  p.slice = ((a.vocab + ctas - 1) / ctas + 15) / 16 * 16;
+  const int own = (kPlaces + ctas - 1) / ctas;
+  const int smem = (kPlaces + 3) / 4 * 16 + own * 12;
+  return launch_clusters(k_sample_values, p, ctas, kValueThreads, smem, st);
+}
+
+template <typename T>
+cudaError_t launch(const LlmqSampleRows &a, int sms, cudaStream_t st) {
+  RowArgs p{};
+  p.a = a;
+  p.scale = scale_bits(a.vocab);
+  // CTAs a row: a slice of at most 64 KB (two CTAs an SM), more while SMs idle
+  int ctas = 1;
+  auto slice_of = [&](int c) { return ((a.vocab + c - 1) / c + 15) / 16 * 16; };
+  while (ctas < kMaxCluster && (slice_of(ctas) * sizeof(T) > 64 * 1024 ||
+                                ((long long)a.n_rows * ctas < 2 * sms && slice_of(ctas) > 2 * kThreads)))
+    ctas *= 2;
+  p.slice = slice_of(ctas);
+  p.resident = p.slice * sizeof(T) <= 160 * 1024;
+  const int smem = kWorkBytes + (p.resident ? p.slice * (int)sizeof(T) : 0);
+  return launch_clusters(k_sample_rows<T>, p, ctas, kThreads, smem, st);
 }
 
 }  // namespace
@@ -796,6 +1325,6 @@ extern "C" LLMQ_API int llmq_sample_rows(const LlmqSampleRows *a, void *stream) 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   c.launched(a->dtype == LLMQ_F32   ? launch<float>(*a, sms, st)
              : a->dtype == LLMQ_F16 ? launch<__half>(*a, sms, st)
-                                    : launch<__nv_bfloat16>(*a, sms, st));
+                                    : launch_values(*a, sms, st));
   return c.rc;
 }
