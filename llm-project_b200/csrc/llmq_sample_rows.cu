@@ -128,6 +128,11 @@ struct Shared {
   int pick_bin, pick_count;
   u64 pick_before, pick_before_count;
   int pick_item;
+  u64 sum;
+  struct {
+    int bin;
+    u64 before, mass;
+  } step[3];  // the top_p cut's, the least and the most the draw can be in
   Command cmd;
 };
 
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   constexpr int kVec = 16 / sizeof(T);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  uint32_t *bin_count = reinterpret_cast<uint32_t *>(s_dyn), *bin_lo = bin_count + kBins, *bin_hi = bin_lo + kBins;
+  uint32_t *bin_count = reinterpret_cast<uint32_t *>(s_dyn), *bin_lo = bin_count + kBins;
   u64 *gathered = reinterpret_cast<u64 *>(s_dyn);
   u64 *tot_mass = reinterpret_cast<u64 *>(s_dyn + kListBytes);
   uint32_t *tot_count = reinterpret_cast<uint32_t *>(tot_mass + kBins);
@@ -219,7 +224,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   const float top_p = a.top_p && a.top_p[r] > 0.0f && a.top_p[r] < 1.0f ? a.top_p[r] : 0.0f;
   const int top_k = a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.vocab ? a.top_k[r] : 0;
 
-  // f(logit, index) for every token of the slice, the next vector on its way meanwhile
+  // f(kVec logits, index of the first) over the slice, the next vector on its way
+  // meanwhile; the ends that fill no vector come one by one, with NaN beside them
   const T *src = p.resident ? slice : row;
   const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));
   const int nv = (n - head) / kVec;
@@ -227,16 +233,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     const Pack<T, kVec> *vec = reinterpret_cast<const Pack<T, kVec> *>(src + head);
     Pack<T, kVec> next;
     if (tid < nv) next = vec[tid];
+    float l[kVec];
     for (int v = tid; v < nv; v += kThreads) {
-      const Pack<T, kVec> x = next;
-      if (v + kThreads < nv) next = vec[v + kThreads];
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) f(to_f32(x.v[i]), j0 + head + v * kVec + i);
+      for (int i = 0; i < kVec; ++i) l[i] = to_f32(next.v[i]);
+      if (v + kThreads < nv) next = vec[v + kThreads];
+      f(l, j0 + head + v * kVec);
     }
-#pragma unroll 1
-    for (int e = tid; e < n - kVec * nv; e += kThreads) {
-      const int j = e < head ? e : e + kVec * nv;
-      f(to_f32(src[j]), j0 + j);
+    const int e = tid < head ? tid : tid + kVec * nv;  // fewer than 2 kVec of them
+    if (tid < n - kVec * nv) {
+#pragma unroll
+      for (int i = 1; i < kVec; ++i) l[i] = NAN;
+      l[0] = to_f32(src[e]);
+      f(l, j0 + e);
     }
   };
 
@@ -254,9 +263,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     __syncthreads();
   }
   float high = -INFINITY, low = INFINITY;  // fmaxf and fminf pass over NaN
-  each([&](float l, int) {
-    high = fmaxf(high, l);
-    low = fminf(low, l);
+  each([&](const float *l, int) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      high = fmaxf(high, l[i]);
+      low = fminf(low, l[i]);
+    }
   });
   const int group_threads = max(1, ctas * kThreads / kGroups), cta_groups = kThreads / group_threads;
   {
@@ -301,8 +313,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   }
   if (greedy) {  // the first of the largest
     int at = INT_MAX;
-    each([&](float l, int j) {
-      if (l == high) at = min(at, j);
+    each([&](const float *l, int j) {
+#pragma unroll
+      for (int i = kVec - 1; i >= 0; --i)
+        if (l[i] == high) at = min(at, j + i);
     });
     at = __reduce_min_sync(0xffffffffu, at);
     if (lane == 0 && at != INT_MAX) atomicMin(&first->pick_item, at);
@@ -369,10 +383,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   // ---- 2. the tokens that reach the bound
   // (at most a few thousand tokens of a row are wanted: one atomic each)
   auto gather = [&](auto wanted) {  // into `gathered`, then to the first CTA's list
-    each([&](float l, int j) {
-      if (wanted(l, j)) {
-        const int at = atomicAdd(&sh.listed, 1);
-        if (at < kListCap) gathered[at] = token_ord(order_key(l), j);
+    each([&](const float *l, int j) {
+      uint32_t want = 0;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) want |= wanted(l[i], j + i) ? 1u << i : 0u;
+      if (want) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          if ((want >> i) & 1u) {
+            const int at = atomicAdd(&sh.listed, 1);
+            if (at < kListCap) gathered[at] = token_ord(order_key(l[i]), j + i);
+          }
       }
     });
     __syncthreads();
@@ -389,48 +410,77 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   if (bounded) {
     const float least = bound > kKeyNegInf ? key_logit(bound) : -FLT_MAX;
     gather([&](float l, int) { return l >= least; });
-    if (top_p > 0.0f) each([&](float l, int) { whole += rule.weight(l); });
+    if (top_p > 0.0f) each([&](const float *l, int) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) whole += rule.weight(l[i]);
+      });
   } else {
     for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
     __syncthreads();
   }
-  auto count_in = [&](u64 w, int b) {
-    if (w == 0) return;  // nothing to any sum
-    const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&bin_lo[b], lo);
-    const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old ? 1u : 0u);
-    if (hi) atomicAdd(&bin_hi[b], hi);
-    if (top_k) atomicAdd(&bin_count[b], 1u);
+  // Adds N weights to their steps: the low words first, all on their way at once, then
+  // the high words with what the low ones carried; nothing for a weight of 0.
+  const uint32_t lo_addr = static_cast<uint32_t>(__cvta_generic_to_shared(bin_lo));
+  auto count_in = [&](const auto &w, const auto &b) {
+    constexpr int N = sizeof(w) / sizeof(w[0]);
+    uint32_t old[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      asm volatile(
+          "{\n\t.reg .pred q;\n\tsetp.ne.u64 q, %3, 0;\n\tmov.u32 %0, 0;\n\t@q atom.shared.add.u32 %0, [%1], %2;\n\t}"
+          : "=&r"(old[i])
+          : "r"(lo_addr + 4 * b[i]), "r"(static_cast<uint32_t>(w[i])), "l"(w[i])
+          : "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t lo = static_cast<uint32_t>(w[i]), hi = static_cast<uint32_t>(w[i] >> 32) + (old[i] + lo < old[i] ? 1u : 0u);
+      asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t@q red.shared.add.u32 [%0], %1;\n\t}" ::"r"(
+                       lo_addr + 4 * (kBins + b[i])),
+                   "r"(hi)
+                   : "memory");
+      if (top_k && w[i]) atomicAdd(&bin_count[b[i]], 1u);
+    }
   };
   auto histogram = [&]() {
-    each([&](float l, int) {
-      const double s = rule.share(l);
-      const u64 w = RowRule::round(s);
-      if (min_p > 0.0f) above += s >= min_share ? w : 0;
-      count_in(w, rule.bin(l));
+    each([&](const float *l, int) {
+#pragma unroll
+      for (int h = 0; h < kVec; h += 4) {
+        u64 w[4];
+        int b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const double s = rule.share(l[h + i]);
+          w[i] = RowRule::round(s);
+          b[i] = rule.bin(l[h + i]);
+          if (min_p > 0.0f) above += s >= min_share ? w[i] : 0;
+        }
+        count_in(w, b);
+      }
     });
   };
-  // the row's histogram in the first CTA, each CTA summing a part of the steps
-  auto collect = [&](u64 *mass, uint32_t *count) {
+  // the row's histogram, each CTA summing a part of the steps: in every CTA, or (of a
+  // divided step) in the first
+  auto collect = [&](u64 *mass, uint32_t *count, int receivers) {
     cluster.sync();
     const int each_bins = kBins / ctas;
-    u64 *m0 = cluster.map_shared_rank(mass, 0);
-    uint32_t *c0 = cluster.map_shared_rank(count, 0);
     for (int i = tid; i < each_bins; i += kThreads) {
       const int b = rank * each_bins + i;
       u64 m = 0;
       uint32_t cnt = 0;
       for (int c = 0; c < ctas; ++c) {
         const uint32_t *h = cluster.map_shared_rank(bin_count, c);
-        cnt += h[b];
         m += h[kBins + b] + (static_cast<u64>(h[2 * kBins + b]) << 32);
+        if (top_k) cnt += h[b];
       }
-      m0[b] = m;
-      c0[b] = cnt;
+      for (int c = 0; c < receivers; ++c) {
+        cluster.map_shared_rank(mass, c)[b] = m;
+        cluster.map_shared_rank(count, c)[b] = cnt;
+      }
     }
   };
   auto publish = [&](u64 v, u64 (Shared::*to)[kMaxCluster]) {
     v = block_sum(v, sh.red);
-    if (tid == 0) (first->*to)[rank] = v;
+    if (tid < ctas) (cluster.map_shared_rank(&sh, tid)->*to)[rank] = v;
   };
   bool have_hist = !bounded;
   if (bounded) {
@@ -441,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     if (!have_hist && rank != 0) return;
     if (have_hist) {
       cluster.barrier_wait();
+      if (rank == 0 && tid == 0) sh.total = 0;  // the next listing comes after the histogram's barriers
       for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
       __syncthreads();
     }
@@ -448,34 +499,44 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   if (have_hist) {
     histogram();
     if (min_p > 0.0f) publish(above, &Shared::above);
-    collect(tot_mass, tot_count);
+    collect(tot_mass, tot_count, ctas);
     cluster.sync();
   }
 
-  // ---- the first CTA decides, the others gather and divide as it says
-  // sorts list[0 .. m) by falling ord, m <= kListCap
+  // sorts list[0 .. m) by falling ord, m <= kListCap (bitonic).  A warp's pairs of a
+  // stride up to 32 stay within its 64 items: only larger strides need the other warps,
+  // and a list of up to 64 items one warp alone.
   auto sort_list = [&](int m) {
     int size2 = 2;
     while (size2 < m) size2 <<= 1;
     for (int i = m + tid; i < size2; i += kThreads) list[i] = 0;
     __syncthreads();
-    for (int size = 2; size <= size2; size <<= 1)
-      for (int stride = size >> 1; stride > 0; stride >>= 1) {
-        for (int i = tid; i < size2 / 2; i += kThreads) {
-          const int x = 2 * i - (i & (stride - 1)), y = x + stride;
-          const u64 u = list[x], v = list[y];
-          if ((u < v) == ((x & size) == 0)) {
-            list[x] = v;
-            list[y] = u;
+    const int warps = max(1, min(kThreads, size2 / 2) / 32);
+    if (warp < warps) {
+      for (int size = 2; size <= size2; size <<= 1)
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+          for (int i = tid; i < size2 / 2; i += 32 * warps) {
+            const int x = 2 * i - (i & (stride - 1)), y = x + stride;
+            const u64 u = list[x], v = list[y];
+            if ((u < v) == ((x & size) == 0)) {
+              list[x] = v;
+              list[y] = u;
+            }
           }
+          if (warps > 1 && (stride > 32 || (stride == 1 && size > 32)))
+            asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
+          else
+            __syncwarp();
         }
-        __syncthreads();
-      }
+    }
+    __syncthreads();
   };
   constexpr int kPer = kListCap / kThreads;
-  // the sorted list's sums: thread's items tid * kPer + i, sum up to and with each
-  auto list_sums = [&](int m, u64 before, u64 *sums) {
-    u64 w[kPer], mine = 0;
+  // a sorted list's weights and sums: thread's items tid * kPer + i, sum up to and with each
+  int m = 0;
+  u64 w[kPer], sums[kPer];
+  auto list_sums = [&](u64 before) {
+    u64 mine = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int x = tid * kPer + i;
@@ -489,25 +550,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       sums[i] = at;
     }
   };
-  // the first of the list's items whose sum reaches target (there is one), and its sum
-  auto reach = [&](int m, const u64 *sums, u64 target, u64 *sum_there) {
-    __syncthreads();
-    if (tid == 0) sh.pick_item = INT_MAX;
-    __syncthreads();
-#pragma unroll
-    for (int i = kPer - 1; i >= 0; --i) {
-      const int x = tid * kPer + i;
-      if (x < m && sums[i] >= target) atomicMin(&sh.pick_item, x);
-    }
-    __syncthreads();
-    const int item = min(sh.pick_item, m - 1);
+  // one thread's item, known to it, and its sum to all
+  auto share_item = [&](auto is_it, u64 *sum_there) -> int {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (tid * kPer + i == item) sh.pick_before = sums[i];
+      if (is_it(i)) {
+        sh.pick_item = tid * kPer + i;
+        sh.pick_before = sums[i];
+      }
     __syncthreads();
     *sum_there = sh.pick_before;
-    return item;
+    return sh.pick_item;
+  };
+  // the first of the list's items whose sum reaches target (there is one), and its sum
+  auto reach = [&](u64 target, u64 *sum_there) {
+    return share_item([&](int i) { return w[i] && sums[i] >= target && sums[i] - w[i] < target; }, sum_there);
   };
   auto answer = [&](int item, u64 kept) {
     if (tid == 0) {
@@ -524,54 +582,120 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   const double u = uf > 0.0f ? fminf(uf, 1.0f) : 0.0f;
 
   if (!have_hist) {  // the list has every cut
-    const int m = sh.total;
-    u64 sums[kPer], there;
+    u64 kept, there;
+    m = sh.total;
     sort_list(m);
-    list_sums(m, 0, sums);
-    u64 kept = ~0ull;
-    if (top_k && top_k < m) {
+    list_sums(0);
+    int cut = top_k && top_k < m ? top_k : m;
+    if (min_p > 0.0f) {  // the items with w >= min_p come first
+      if (tid == 0) sh.pick_count = 0;
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (tid * kPer + i == top_k - 1) sh.pick_before = sums[i];
-      __syncthreads();
-      kept = sh.pick_before;
-    }
-    {  // the last item, or the last with w >= min_p
-      int last = 0;
+      int c = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int x = tid * kPer + i;
-        if (x < m && rule.share(key_logit(static_cast<uint32_t>(list[x] >> kIndexBits))) >= min_share) last = x + 1;
+        c += x < m && rule.share(key_logit(static_cast<uint32_t>(list[x] >> kIndexBits))) >= min_share;
       }
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (lane == 0 && c) atomicAdd(&sh.pick_count, c);
       __syncthreads();
-      if (tid == 0) sh.pick_item = 0;
-      __syncthreads();
-      if (last) atomicMax(&sh.pick_item, last);
-      __syncthreads();
-      const int item = sh.pick_item - 1;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (tid * kPer + i == item) sh.pick_before = sums[i];
-      __syncthreads();
-      kept = min(kept, sh.pick_before);
+      cut = min(cut, sh.pick_count);
     }
+    share_item([&](int i) { return tid * kPer + i == cut - 1; }, &kept);
     if (top_p > 0.0f) {
       u64 z = 0;
       for (int c = 0; c < ctas; ++c) z += sh.whole[c];
       const u64 target = part_of(top_p, z);
       if (target < kept) {  // reached within the list
-        reach(m, sums, target, &there);
-        kept = min(kept, there);
+        reach(target, &there);
+        kept = there;
       }
     }
-    const int item = reach(m, sums, part_of(u, kept), &there);
+    const int item = reach(part_of(u, kept), &there);
     answer(item, kept);
     cluster.barrier_wait();
     return;
   }
 
+  // ---- 3. by the histogram
+  u64 z = 0, kept = 0;
+  {
+    // Without a top_k every CTA finds the step of the top_p cut and, as that bounds what
+    // is kept from both sides, the one or two steps the draw can be in; all are listed at
+    // once.
+    u64 mass[kBins / kThreads], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kBins / kThreads; ++i) {
+      mass[i] = tot_mass[tid * (kBins / kThreads) + i];
+      mine += mass[i];
+    }
+    const u64 upto = block_scan(mine, sh.red);
+    if (tid == kThreads - 1) sh.sum = upto;
+    __syncthreads();
+    z = sh.sum;
+    if (min_p > 0.0f)
+      for (int c = 0; c < ctas; ++c) kept += sh.above[c];
+    else
+      kept = z;
+    if (!top_k) {
+      auto locate = [&](int which, u64 target) {
+        u64 at = upto - mine;
+#pragma unroll
+        for (int i = 0; i < kBins / kThreads; ++i) {
+          if (at < target && at + mass[i] >= target) {
+            sh.step[which].bin = tid * (kBins / kThreads) + i;
+            sh.step[which].before = at;
+            sh.step[which].mass = mass[i];
+          }
+          at += mass[i];
+        }
+      };
+      const u64 cut = top_p > 0.0f ? part_of(top_p, z) : kept;
+      const bool cuts = cut < kept;
+      u64 most = kept;
+      if (cuts) {
+        locate(0, cut);
+        __syncthreads();
+        most = min(kept, sh.step[0].before + sh.step[0].mass);
+      }
+      locate(1, part_of(u, cuts ? cut : kept));
+      locate(2, part_of(u, most));
+      __syncthreads();
+      const int b0 = sh.step[1].bin, b1 = sh.step[2].bin, bp = cuts ? sh.step[0].bin : b1;
+      gather([&](float l, int) {
+        const int b = rule.bin(l);
+        return ((b >= b0 && b <= b1) || b == bp) && l > -INFINITY;
+      });
+      cluster.sync();
+      const bool overflow = first->total > kListCap;
+      cluster.barrier_arrive();  // the first CTA outlives the others' look at its memory
+      if (!overflow && rank != 0) return;
+      if (!overflow) {
+        m = sh.total;
+        sort_list(m);
+        list_sums(sh.step[1].before);
+        // the cut's step, where it is apart, goes on from its own sum
+        const u64 gap = bp > b1 ? sh.step[0].before - (sh.step[2].before + sh.step[2].mass) : 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int x = tid * kPer + i;
+          if (x < m && rule.bin(key_logit(static_cast<uint32_t>(list[x] >> kIndexBits))) > b1) sums[i] += gap;
+        }
+        u64 there;
+        if (cuts) {
+          reach(cut, &there);
+          kept = min(kept, there);
+        }
+        const int item = reach(part_of(u, kept), &there);
+        answer(item, kept);
+        cluster.barrier_wait();
+        return;
+      }
+      cluster.barrier_wait();
+    }
+  }
+
+  // ---- otherwise the first CTA decides, the others gather and divide as it says
   // the tokens of a command's steps and range
   auto in_command = [&](const Command &c, float l, int j) {
     const int b = rule.bin(l);
@@ -591,12 +715,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     } else {
       for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
       __syncthreads();
-      each([&](float l, int j) {
-        if (!in_command(c, l, j)) return;
-        const u64 w = rule.weight(l), s = (c.hi - token_ord(order_key(l), j)) >> c.shift;
-        count_in(w, static_cast<int>(min(s, (u64)(kBins - 1))));
+      each([&](const float *l, int j) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          if (!in_command(c, l[i], j + i)) continue;
+          const u64 w[1] = {rule.weight(l[i])}, s = (c.hi - token_ord(order_key(l[i]), j + i)) >> c.shift;
+          const int b[1] = {static_cast<int>(min(s, (u64)(kBins - 1)))};
+          count_in(w, b);
+        }
       });
-      collect(list, reinterpret_cast<uint32_t *>(list + kBins));
+      collect(list, reinterpret_cast<uint32_t *>(list + kBins), 1);
     }
     cluster.sync();
     return true;
@@ -636,8 +764,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   // Lists the tokens around where the measure reaches target; returns the item there,
   // *sum_there the row's sum up to and with it.  If all tokens up to there fit the
   // list, they are listed and *from_start is set.
-  int m = 0;
-  u64 sums[kPer];
   auto select = [&](bool by_count, u64 target, bool *from_start, u64 *sum_there) {
     find_step(tot_mass, tot_count, by_count, target, 0, 0);
     Command c{};
@@ -695,30 +821,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     }
     m = min(sh.total, kListCap);
     sort_list(m);
-    list_sums(m, before, sums);
+    list_sums(before);
     if (by_count) {
       const int item = min(static_cast<int>(target - before_n) - 1, m - 1);
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (tid * kPer + i == item) sh.pick_before = sums[i];
-      __syncthreads();
-      *sum_there = sh.pick_before;
-      return item;
+      return share_item([&](int i) { return tid * kPer + i == item; }, sum_there);
     }
-    return reach(m, sums, target, sum_there);
+    return reach(target, sum_there);
   };
-  u64 z = 0, kept = 0, tokens = 0;
-  for (int b = tid; b < kBins; b += kThreads) {
-    z += tot_mass[b];
-    tokens += tot_count[b];
+  u64 tokens = 0;
+  if (top_k) {
+    for (int b = tid; b < kBins; b += kThreads) tokens += tot_count[b];
+    tokens = block_sum(tokens, sh.red);
   }
-  z = block_sum(z, sh.red);
-  tokens = top_k ? block_sum(tokens, sh.red) : 0;
-  if (min_p > 0.0f)
-    for (int c = 0; c < ctas; ++c) kept += sh.above[c];
-  else
-    kept = z;
   bool from_start = false;
   u64 there;
   if (top_k && static_cast<u64>(top_k) < tokens) {
@@ -729,7 +843,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     const u64 target = part_of(top_p, z);
     if (target < kept) {
       if (from_start)
-        reach(m, sums, target, &there);
+        reach(target, &there);
       else
         select(false, target, &from_start, &there);
       kept = min(kept, there);
@@ -738,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   const u64 target = part_of(u, kept);
   int item;
   if (from_start)
-    item = reach(m, sums, target, &there);
+    item = reach(target, &there);
   else
     item = select(false, target, &from_start, &there);
   answer(item, kept);
