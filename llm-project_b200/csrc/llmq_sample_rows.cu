@@ -12,17 +12,19 @@
 // times the kept one.  No cut needs a sorted row: only the tokens around it.
 //
 // A cluster of CTAs holds a row in shared memory, read from DRAM once:
-//  1. The largest and least logit, and for a small top_k the largest of each of
-//     some thousand groups of tokens: the k-th largest of those is a bound that at
-//     least k tokens reach and few more do (k = 40: about 41 of a smooth row's).  A
-//     min_p gives another bound.
+//  1. The largest and least logit, and for a top_k up to 96 the largest of each of
+//     128 groups of tokens: the k-th largest of those is a bound that at least k
+//     tokens reach and few more do (k = 40: about 48 of a smooth row's).  A min_p
+//     gives another bound.
 //  2. With a bound, the tokens that reach it go to the first CTA's list (the whole
 //     sum, where top_p asks for it, is formed on the way).  The list is sorted and
 //     everything follows from its prefix sums.
-//  3. Without one (or if the list overflows), a histogram of counts and exact
-//     sums over kBins steps of the logit; each cut, then the draw, finds its step by
-//     a prefix sum and lists that step's tokens alone.  A step with too many tokens
-//     is divided again, by ord, down to single tokens if need be (rows of ties).
+//  3. Without one (or if the list overflows), a histogram of exact sums (and counts,
+//     for a top_k) over kBins steps of the logit.  A prefix sum finds the step each
+//     cut lies in, which bounds the kept sum and so the steps the draw can be in; the
+//     tokens of these few steps are listed and sorted.  If they are too many (rows of
+//     ties), the cuts and the draw go one by one, dividing a step by ord, down to
+//     single tokens if need be.
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -40,7 +42,7 @@ constexpr int kThreads = 512;
 constexpr int kBins = 1024;
 constexpr int kListCap = 2048;
 constexpr int kMaxCluster = 8;
-constexpr int kGroups = 2048;  // groups of tokens whose maxima bound a top_k
+constexpr int kGroups = 128;  // groups of tokens whose maxima bound a top_k
 constexpr int kIndexBits = 20;
 
 __device__ __forceinline__ uint32_t order_key(float l) {
@@ -114,6 +116,12 @@ struct Command {
 };
 enum { kDone = 0, kGather = 1, kDivide = 2 };
 
+// A step of the histogram: its sum and tokens, and those before it.
+struct Step {
+  int bin, before_n, count;
+  u64 before, mass;
+};
+
 // What each CTA keeps in static shared memory; the first CTA's is the row's.
 struct Shared {
   double tab[kExpTable];
@@ -123,16 +131,13 @@ struct Shared {
   int listed;        // tokens gathered here
   int total;         // the row's list (first CTA)
   int place;         // where this CTA's part of it goes
-  unsigned digits[256];
+  __align__(16) uint32_t groups[kGroups];
   uint32_t pick_key;
   int pick_bin, pick_count;
   u64 pick_before, pick_before_count;
   int pick_item;
-  u64 sum;
-  struct {
-    int bin;
-    u64 before, mass;
-  } step[3];  // the top_p cut's, the least and the most the draw can be in
+  u64 sum, tokens;
+  Step step[4];  // the top_p cut's, the top_k's, the least and the most the draw can be in
   Command cmd;
 };
 
@@ -181,7 +186,7 @@ __device__ __forceinline__ u64 part_of(double f, u64 total) {
 constexpr int kHistBytes = kBins * 12;
 constexpr int kListBytes = kListCap * 8;
 constexpr int kWorkBytes = kListBytes + kHistBytes + kListBytes;
-static_assert(kHistBytes <= kListBytes && kGroups * 4 <= kHistBytes, "regions are shared");
+static_assert(kHistBytes <= kListBytes, "regions are shared");
 
 struct RowArgs {
   LlmqSampleRows a;
@@ -202,7 +207,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   u64 *tot_mass = reinterpret_cast<u64 *>(s_dyn + kListBytes);
   uint32_t *tot_count = reinterpret_cast<uint32_t *>(tot_mass + kBins);
   u64 *list = reinterpret_cast<u64 *>(s_dyn + kListBytes + kHistBytes);
-  uint32_t *groups = reinterpret_cast<uint32_t *>(tot_mass);  // read before any CTA can be at a histogram's sums
   T *slice = reinterpret_cast<T *>(s_dyn + kWorkBytes);
   Shared *first = cluster.map_shared_rank(&sh, 0);
 
@@ -270,10 +274,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       low = fminf(low, l[i]);
     }
   });
-  const int group_threads = max(1, ctas * kThreads / kGroups), cta_groups = kThreads / group_threads;
   {
+    const int lanes = ctas * kThreads / kGroups;  // of a group: 4 .. 32
     float g = high;
-    for (int o = 1; o < group_threads; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    for (int o = 1; o < lanes; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
     float hi = high, lo = low;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -286,9 +290,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     }
     __syncthreads();
     cluster.barrier_wait();
-    if (top_k && !greedy && tid % group_threads == 0)
+    if (top_k && tid % lanes == 0)
       for (int c = 0; c < ctas; ++c)
-        cluster.map_shared_rank(groups, c)[rank * cta_groups + tid / group_threads] = order_key(g);
+        cluster.map_shared_rank(&sh, c)->groups[(rank * kThreads + tid) / lanes] = order_key(g);
     if (tid < ctas) {
       for (int w = 0; w < kThreads / 32; ++w) {
         hi = fmaxf(hi, sh.warp_high[w]);
@@ -339,36 +343,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   // ---- a bound that the tokens of every cut reach
   uint32_t bound = 0;
   bool bounded = a.vocab <= kListCap;
-  if (!bounded && top_k && top_k <= ctas * cta_groups * 3 / 4) {
-    // the top_k-th largest of the groups' maxima, by digits of 8 bits
-    const int ng = ctas * cta_groups;
-    uint32_t prefix = 0, mask = 0;
-    int rest = top_k;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) sh.digits[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < ng; i += kThreads)
-        if ((groups[i] & mask) == prefix) atomicAdd(&sh.digits[(groups[i] >> shift) & 255u], 1u);
-      __syncthreads();
-      if (warp == 0) {
-        // lane: digits 255 - 8 lane down to 248 - 8 lane
-        int sum = 0;
-        for (int i = 0; i < 8; ++i) sum += sh.digits[255 - 8 * lane - i];
-        const int incl = static_cast<int>(warp_scan(sum));
-        const unsigned who = __ballot_sync(0xffffffffu, incl >= rest);
-        if (lane == __ffs(who) - 1) {
-          int before = incl - sum, d = 255 - 8 * lane;
-          while (before + static_cast<int>(sh.digits[d]) < rest) before += sh.digits[d--];
-          sh.pick_key = prefix | (static_cast<uint32_t>(d) << shift);
-          sh.pick_count = rest - before;
-        }
-      }
-      __syncthreads();
-      prefix = sh.pick_key;
-      rest = sh.pick_count;
-      mask |= 255u << shift;
+  if (!bounded && top_k && top_k <= kGroups * 3 / 4) {
+    // the top_k-th largest of the groups' maxima: four threads count what precedes each
+    constexpr int kParts = kThreads / kGroups;
+    const int g = tid / kParts, part = tid % kParts;
+    const uint32_t mine = sh.groups[g];
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups / kParts; ++i) {
+      const int x = part + kParts * i;
+      const uint32_t k = sh.groups[x];
+      before += k > mine || (k == mine && x < g);
     }
-    bound = prefix;
+    for (int o = 1; o < kParts; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (before == top_k - 1) sh.pick_key = mine;
+    __syncthreads();
+    bound = sh.pick_key;
     bounded = true;
   }
   if (min_p > 0.0f) {
@@ -378,19 +368,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     bound = max(bound, min(k, order_key(high)));
     bounded = true;
   }
-  __syncthreads();  // the groups have been read
 
   // ---- 2. the tokens that reach the bound
-  // (at most a few thousand tokens of a row are wanted: one atomic each)
-  auto gather = [&](auto wanted) {  // into `gathered`, then to the first CTA's list
+  // Lists what is wanted of the logits in [lo, hi] (a first, cheap look), at most a few
+  // thousand tokens of a row, one atomic each: into `gathered`, then to the first
+  // CTA's list.
+  auto gather = [&](float lo, float hi, auto wanted) {
     each([&](const float *l, int j) {
       uint32_t want = 0;
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) want |= wanted(l[i], j + i) ? 1u << i : 0u;
+      for (int i = 0; i < kVec; ++i) want |= l[i] >= lo && l[i] <= hi ? 1u << i : 0u;
       if (want) {
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
-          if ((want >> i) & 1u) {
+          if (((want >> i) & 1u) && wanted(l[i], j + i)) {
             const int at = atomicAdd(&sh.listed, 1);
             if (at < kListCap) gathered[at] = token_ord(order_key(l[i]), j + i);
           }
@@ -405,11 +396,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       if (sh.place + i < kListCap) to[sh.place + i] = gathered[i];
     if (tid == 0) sh.listed = 0;
   };
+  // logits that all tokens of steps b0 .. b1 lie between
+  const float width = rule.bin_scale > 0.0f ? 1.0f / rule.bin_scale : INFINITY;
+  auto over_step = [&](int b) { return b > 0 && width < INFINITY ? high - width * static_cast<float>(b - 1) : INFINITY; };
+  auto under_step = [&](int b) {
+    return b < kBins - 1 && width < INFINITY ? fmaxf(high - width * static_cast<float>(b + 1), -FLT_MAX) : -FLT_MAX;
+  };
   const double min_share = ldexp(static_cast<double>(min_p), p.scale);
   u64 whole = 0, above = 0;
   if (bounded) {
     const float least = bound > kKeyNegInf ? key_logit(bound) : -FLT_MAX;
-    gather([&](float l, int) { return l >= least; });
+    gather(least, INFINITY, [](float, int) { return true; });
     if (top_p > 0.0f) each([&](const float *l, int) {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) whole += rule.weight(l[i]);
@@ -506,7 +503,27 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   // sorts list[0 .. m) by falling ord, m <= kListCap (bitonic).  A warp's pairs of a
   // stride up to 32 stay within its 64 items: only larger strides need the other warps,
   // and a list of up to 64 items one warp alone.
+  // Up to kThreads items are put in place by counting what precedes each, several
+  // threads an item; the sorted items are then in `gathered`.
+  u64 *items = list;
   auto sort_list = [&](int m) {
+    if (m <= kThreads) {
+      int parts = 1;  // threads an item, 32 at most
+      while (parts < 32 && m * parts * 2 <= kThreads) parts *= 2;
+      const int x = tid / parts;
+      int before = 0;
+      if (x < m) {
+        const u64 mine = list[x];
+#pragma unroll 4
+        for (int y = tid % parts; y < m; y += parts) before += list[y] > mine;
+      }
+      for (int o = 1; o < parts; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+      items = gathered;
+      if (x < m && tid % parts == 0) items[before] = list[x];
+      __syncthreads();
+      return;
+    }
+    items = list;
     int size2 = 2;
     while (size2 < m) size2 <<= 1;
     for (int i = m + tid; i < size2; i += kThreads) list[i] = 0;
@@ -540,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int x = tid * kPer + i;
-      w[i] = x < m ? rule.weight(key_logit(static_cast<uint32_t>(list[x] >> kIndexBits))) : 0;
+      w[i] = x < m ? rule.weight(key_logit(static_cast<uint32_t>(items[x] >> kIndexBits))) : 0;
       mine += w[i];
     }
     u64 at = before + block_scan(mine, sh.red) - mine;
@@ -569,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   };
   auto answer = [&](int item, u64 kept) {
     if (tid == 0) {
-      const u64 o = list[item];
+      const u64 o = items[item];
       const float l = key_logit(static_cast<uint32_t>(o >> kIndexBits));
       a.ids[r] = (1 << kIndexBits) - 1 - static_cast<int>(o & ((1 << kIndexBits) - 1));
       if (a.logprobs) {
@@ -594,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int x = tid * kPer + i;
-        c += x < m && rule.share(key_logit(static_cast<uint32_t>(list[x] >> kIndexBits))) >= min_share;
+        c += x < m && rule.share(key_logit(static_cast<uint32_t>(items[x] >> kIndexBits))) >= min_share;
       }
       c = __reduce_add_sync(0xffffffffu, c);
       if (lane == 0 && c) atomicAdd(&sh.pick_count, c);
@@ -618,81 +635,124 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   }
 
   // ---- 3. by the histogram
-  u64 z = 0, kept = 0;
+  u64 z = 0, kept = 0, tokens = 0;
   {
-    // Without a top_k every CTA finds the step of the top_p cut and, as that bounds what
-    // is kept from both sides, the one or two steps the draw can be in; all are listed at
-    // once.
-    u64 mass[kBins / kThreads], mine = 0;
+    // Every CTA finds the steps of the cuts and, as those bound what is kept from both
+    // sides, the one or two steps the draw can be in; all are listed at once.
+    constexpr int kOwn = kBins / kThreads;
+    u64 mass[kOwn], mine = 0;
+    uint32_t count[kOwn], mine_n = 0;
 #pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) {
-      mass[i] = tot_mass[tid * (kBins / kThreads) + i];
+    for (int i = 0; i < kOwn; ++i) {
+      mass[i] = tot_mass[tid * kOwn + i];
+      count[i] = top_k ? tot_count[tid * kOwn + i] : 0;
       mine += mass[i];
+      mine_n += count[i];
     }
-    const u64 upto = block_scan(mine, sh.red);
-    if (tid == kThreads - 1) sh.sum = upto;
+    const u64 upto = block_scan(mine, sh.red), upto_n = top_k ? block_scan(mine_n, sh.red) : 0;
+    if (tid == kThreads - 1) {
+      sh.sum = upto;
+      sh.tokens = upto_n;
+    }
     __syncthreads();
     z = sh.sum;
+    tokens = sh.tokens;
     if (min_p > 0.0f)
       for (int c = 0; c < ctas; ++c) kept += sh.above[c];
     else
       kept = z;
-    if (!top_k) {
-      auto locate = [&](int which, u64 target) {
-        u64 at = upto - mine;
+    auto locate = [&](int which, bool by_count, u64 target) {
+      u64 at = upto - mine, at_n = upto_n - mine_n;
 #pragma unroll
-        for (int i = 0; i < kBins / kThreads; ++i) {
-          if (at < target && at + mass[i] >= target) {
-            sh.step[which].bin = tid * (kBins / kThreads) + i;
-            sh.step[which].before = at;
-            sh.step[which].mass = mass[i];
-          }
-          at += mass[i];
+      for (int i = 0; i < kOwn; ++i) {
+        const u64 has = by_count ? at_n : at, gets = has + (by_count ? count[i] : mass[i]);
+        if (has < target && gets >= target) {
+          Step &t = sh.step[which];
+          t.bin = tid * kOwn + i;
+          t.before = at;
+          t.mass = mass[i];
+          t.before_n = static_cast<int>(at_n);
+          t.count = static_cast<int>(count[i]);
         }
-      };
-      const u64 cut = top_p > 0.0f ? part_of(top_p, z) : kept;
-      const bool cuts = cut < kept;
-      u64 most = kept;
-      if (cuts) {
-        locate(0, cut);
-        __syncthreads();
-        most = min(kept, sh.step[0].before + sh.step[0].mass);
+        at += mass[i];
+        at_n += count[i];
       }
-      locate(1, part_of(u, cuts ? cut : kept));
-      locate(2, part_of(u, most));
-      __syncthreads();
-      const int b0 = sh.step[1].bin, b1 = sh.step[2].bin, bp = cuts ? sh.step[0].bin : b1;
-      gather([&](float l, int) {
-        const int b = rule.bin(l);
-        return ((b >= b0 && b <= b1) || b == bp) && l > -INFINITY;
-      });
-      cluster.sync();
-      const bool overflow = first->total > kListCap;
-      cluster.barrier_arrive();  // the first CTA outlives the others' look at its memory
-      if (!overflow && rank != 0) return;
-      if (!overflow) {
-        m = sh.total;
-        sort_list(m);
-        list_sums(sh.step[1].before);
-        // the cut's step, where it is apart, goes on from its own sum
-        const u64 gap = bp > b1 ? sh.step[0].before - (sh.step[2].before + sh.step[2].mass) : 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int x = tid * kPer + i;
-          if (x < m && rule.bin(key_logit(static_cast<uint32_t>(list[x] >> kIndexBits))) > b1) sums[i] += gap;
-        }
-        u64 there;
-        if (cuts) {
-          reach(cut, &there);
-          kept = min(kept, there);
-        }
-        const int item = reach(part_of(u, kept), &there);
-        answer(item, kept);
-        cluster.barrier_wait();
-        return;
-      }
-      cluster.barrier_wait();
+    };
+    const u64 cut = top_p > 0.0f ? part_of(top_p, z) : kept;
+    const bool cuts_p = cut < kept, cuts_k = top_k && static_cast<u64>(top_k) < tokens;
+    if (cuts_p) locate(0, false, cut);
+    if (cuts_k) locate(1, true, top_k);
+    __syncthreads();
+    const Step sp = sh.step[0], sk = sh.step[1];
+    u64 fewest = kept, most = kept;
+    if (cuts_p) {
+      fewest = cut;
+      most = min(most, sp.before + sp.mass);
     }
+    if (cuts_k) {
+      fewest = min(fewest, sk.before + 1);
+      most = min(most, sk.before + sk.mass);
+    }
+    locate(2, false, part_of(u, fewest));
+    locate(3, false, part_of(u, most));
+    __syncthreads();
+    const Step s0 = sh.step[2], s1 = sh.step[3];
+    // the cuts' steps that lie behind the draw's, in order (kBins: none)
+    int c0 = cuts_p && sp.bin > s1.bin ? sp.bin : kBins, c1 = cuts_k && sk.bin > s1.bin && sk.bin != c0 ? sk.bin : kBins;
+    if (c1 < c0) {
+      const int t = c0;
+      c0 = c1;
+      c1 = t;
+    }
+    const int last = c1 < kBins ? c1 : c0 < kBins ? c0 : s1.bin;
+    gather(under_step(last), over_step(s0.bin), [&](float l, int) {
+      const int b = rule.bin(l);
+      return (b >= s0.bin && b <= s1.bin) || b == c0 || b == c1;
+    });
+    cluster.sync();
+    const bool overflow = first->total > kListCap;
+    cluster.barrier_arrive();  // the first CTA outlives the others' look at its memory
+    if (!overflow) {
+      if (rank != 0) return;
+      m = sh.total;
+      sort_list(m);
+      list_sums(s0.before);
+      // a cut's step that lies apart goes on from its own sum and count
+      const u64 end = s1.before + s1.mass;
+      const int end_n = s1.before_n + s1.count;
+      const Step &t0 = cuts_p && c0 == sp.bin ? sp : sk, &t1 = cuts_p && c1 == sp.bin ? sp : sk;
+      int skipped[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int x = tid * kPer + i;
+        skipped[i] = s0.before_n;
+        if (x < m) {
+          const int b = rule.bin(key_logit(static_cast<uint32_t>(items[x] >> kIndexBits)));
+          if (b > s1.bin) {
+            sums[i] += t0.before - end;
+            skipped[i] += t0.before_n - end_n;
+          }
+          if (b > c0) {
+            sums[i] += t1.before - (t0.before + t0.mass);
+            skipped[i] += t1.before_n - (t0.before_n + t0.count);
+          }
+        }
+      }
+      u64 there;
+      if (cuts_k) {
+        share_item([&](int i) { return tid * kPer + i < m && tid * kPer + i + 1 + skipped[i] == top_k; }, &there);
+        kept = min(kept, there);
+      }
+      if (cuts_p) {
+        reach(cut, &there);
+        kept = min(kept, there);
+      }
+      const int item = reach(part_of(u, kept), &there);
+      answer(item, kept);
+      cluster.barrier_wait();
+      return;
+    }
+    cluster.barrier_wait();
   }
 
   // ---- otherwise the first CTA decides, the others gather and divide as it says
@@ -711,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       return false;
     }
     if (c.op == kGather) {
-      gather([&](float l, int j) { return in_command(c, l, j); });
+      gather(-FLT_MAX, INFINITY, [&](float l, int j) { return in_command(c, l, j); });
     } else {
       for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
       __syncthreads();
@@ -828,11 +888,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     }
     return reach(target, sum_there);
   };
-  u64 tokens = 0;
-  if (top_k) {
-    for (int b = tid; b < kBins; b += kThreads) tokens += tot_count[b];
-    tokens = block_sum(tokens, sh.red);
-  }
   bool from_start = false;
   u64 there;
   if (top_k && static_cast<u64>(top_k) < tokens) {
