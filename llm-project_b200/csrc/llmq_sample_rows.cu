@@ -29,6 +29,7 @@
 #include <climits>
 #include <cmath>
 #include <cooperative_groups.h>
+#include <type_traits>
 
 #include "llmq_serve.cuh"
 
@@ -67,12 +68,14 @@ struct RowRule {
   bool infinite;       // it is +infinity: only its equals count, whatever T
   double mxd, step;    // step: 256 log2(e) / T
   int scale;           // S
-  const double *tab;   // shared
+  const double *tab;   // shared: 2^(S - i / 256)
   float bin_scale;     // steps of the histogram a unit of logit
 
-  // w * 2^S before rounding; 0 for NaN and -infinity
-  __device__ __forceinline__ double share(float l) const {
-    if (infinite) return l == mx ? __hiloint2double((1023 + scale) << 20, 0) : 0.0;
+  uint32_t far;        // high word of 256 (S + 1): a y from there on has a w that rounds to 0
+
+  // w * 2^S before rounding; *counts: it does not round to 0 (false for NaN and
+  // -infinity; the value is then nothing).  Not for an infinite maximum.
+  __device__ __forceinline__ double share_near(float l, bool *counts) const {
     const double y = (mxd - static_cast<double>(l)) * step;  // >= 0, or NaN
     const double yr = y + 6755399441055744.0;  // 1.5 * 2^52: the integer in the low bits
     const int n = __double2loint(yr);
@@ -82,9 +85,15 @@ struct RowRule {
     p = fma(x, p, c * c / 2.0);
     p = fma(x, p, c);
     p = fma(x, p, 1.0);
-    const double t = tab[n & (kExpTable - 1)];
-    const double s = p * __hiloint2double(__double2hiint(t) + ((scale - (n >> 8)) << 20), __double2loint(t));
-    return static_cast<uint32_t>(__double2hiint(y)) < 0x40cf8000u ? s : 0.0;  // y < 16128 (2^-63), no NaN of either sign
+    const double t = tab[n & (kExpTable - 1)];  // of 2^S 2^(-i / 256)
+    *counts = static_cast<uint32_t>(__double2hiint(y)) < far;  // as unsigned: no NaN of either sign
+    return p * __hiloint2double(__double2hiint(t) - ((n >> 8) << 20), __double2loint(t));
+  }
+  __device__ __forceinline__ double share(float l) const {
+    if (infinite) return l == mx ? __hiloint2double((1023 + scale) << 20, 0) : 0.0;
+    bool counts;
+    const double s = share_near(l, &counts);
+    return counts ? s : 0.0;
   }
   static __device__ __forceinline__ u64 round(double s) {
     const double r = s + 6755399441055744.0;  // s < 2^51
@@ -103,6 +112,7 @@ struct RowRule {
     mxd = static_cast<double>(mx);
     step = kExpTable * 1.4426950408889634 / static_cast<double>(temp);
     scale = bits;
+    far = static_cast<uint32_t>(__double2hiint(kExpTable * static_cast<double>(bits + 1)));
     tab = table;
     bin_scale = 0.0f;
   }
@@ -214,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x / ctas, j0 = rank * p.slice, n = max(0, min(p.slice, a.vocab - j0));
   cluster.barrier_arrive();  // every CTA runs before any writes to another
-  if (tid < kExpTable) sh.tab[tid] = exp2(-tid / static_cast<double>(kExpTable));
+  if (tid < kExpTable) sh.tab[tid] = exp2(p.scale - tid * (1.0 / kExpTable));
   if (tid == 0) {
     sh.listed = sh.total = 0;
     sh.pick_item = INT_MAX;
@@ -274,6 +284,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       low = fminf(low, l[i]);
     }
   });
+  const float thread_high = high;
   {
     const int lanes = ctas * kThreads / kGroups;  // of a group: 4 .. 32
     float g = high;
@@ -402,12 +413,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   auto under_step = [&](int b) {
     return b < kBins - 1 && width < INFINITY ? fmaxf(high - width * static_cast<float>(b + 1), -FLT_MAX) : -FLT_MAX;
   };
-  const double min_share = ldexp(static_cast<double>(min_p), p.scale);
+  const double min_share = static_cast<double>(min_p) * static_cast<double>(1ull << p.scale);
   u64 whole = 0, above = 0;
   if (bounded) {
     const float least = bound > kKeyNegInf ? key_logit(bound) : -FLT_MAX;
-    gather(least, INFINITY, [](float, int) { return true; });
-    if (top_p > 0.0f) each([&](const float *l, int) {
+    // A min_p says nothing of how many tokens reach it.  Of kThreads threads with a share
+    // of the slice each, `over` have one that does: some -kThreads ln(1 - over / kThreads)
+    // tokens.  Half again too many for the list: it overflows without being tried.
+    const int over = __syncthreads_count(thread_high >= least);
+    const bool hopeless = a.vocab > kListCap &&
+                          -kThreads * logf(1.0f - over / (kThreads + 0.5f)) > 1.5f * kListCap / ctas;
+    if (hopeless && tid == 0) atomicAdd(&first->total, kListCap + 1);
+    if (!hopeless) gather(least, INFINITY, [](float, int) { return true; });
+    if (top_p > 0.0f && !hopeless) each([&](const float *l, int) {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) whole += rule.weight(l[i]);
       });
@@ -415,45 +433,58 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     for (int b = tid; b < 3 * kBins; b += kThreads) bin_count[b] = 0;
     __syncthreads();
   }
-  // Adds N weights to their steps: the low words first, all on their way at once, then
-  // the high words with what the low ones carried; nothing for a weight of 0.
+  // Adds N weights to their steps, those that count: the low words first, all on their
+  // way at once, then the high words with what the low ones carried.
   const uint32_t lo_addr = static_cast<uint32_t>(__cvta_generic_to_shared(bin_lo));
-  auto count_in = [&](const auto &w, const auto &b) {
+  auto count_in = [&](const auto &w, const auto &b, const auto &counts, auto counted) {
     constexpr int N = sizeof(w) / sizeof(w[0]);
     uint32_t old[N];
 #pragma unroll
     for (int i = 0; i < N; ++i)
       asm volatile(
-          "{\n\t.reg .pred q;\n\tsetp.ne.u64 q, %3, 0;\n\tmov.u32 %0, 0;\n\t@q atom.shared.add.u32 %0, [%1], %2;\n\t}"
+          "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %3, 0;\n\t@q atom.shared.add.u32 %0, [%1], %2;\n\t}"
           : "=&r"(old[i])
-          : "r"(lo_addr + 4 * b[i]), "r"(static_cast<uint32_t>(w[i])), "l"(w[i])
+          : "r"(lo_addr + 4 * b[i]), "r"(static_cast<uint32_t>(w[i])), "r"(counts[i] ? 1u : 0u)
           : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint32_t lo = static_cast<uint32_t>(w[i]), hi = static_cast<uint32_t>(w[i] >> 32) + (old[i] + lo < old[i] ? 1u : 0u);
-      asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t@q red.shared.add.u32 [%0], %1;\n\t}" ::"r"(
-                       lo_addr + 4 * (kBins + b[i])),
-                   "r"(hi)
+      asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q red.shared.add.u32 [%0+%3], %1;\n\t}" ::"r"(
+                       lo_addr + 4 * b[i]),
+                   "r"(hi), "r"(counts[i] ? hi : 0u), "n"(4 * kBins)
                    : "memory");
-      if (top_k && w[i]) atomicAdd(&bin_count[b[i]], 1u);
+      if (counted.value && counts[i]) atomicAdd(&bin_count[b[i]], 1u);
     }
   };
-  auto histogram = [&]() {
+  // `all`: with counts (of a top_k) and the sum of w >= min_p, for any maximum
+  auto fill = [&](auto all) {
     each([&](const float *l, int) {
 #pragma unroll
       for (int h = 0; h < kVec; h += 4) {
         u64 w[4];
         int b[4];
+        bool counts[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const double s = rule.share(l[h + i]);
-          w[i] = RowRule::round(s);
+          if (all.value) {
+            const double s = rule.share(l[h + i]);
+            w[i] = RowRule::round(s);
+            counts[i] = w[i] != 0;
+            above += s >= min_share ? w[i] : 0;
+          } else {
+            w[i] = RowRule::round(rule.share_near(l[h + i], &counts[i]));
+          }
           b[i] = rule.bin(l[h + i]);
-          if (min_p > 0.0f) above += s >= min_share ? w[i] : 0;
         }
-        count_in(w, b);
+        count_in(w, b, counts, all);
       }
     });
+  };
+  auto histogram = [&]() {
+    if (top_k || min_p > 0.0f || rule.infinite)
+      fill(std::true_type());
+    else
+      fill(std::false_type());
   };
   // the row's histogram, each CTA summing a part of the steps: in every CTA, or (of a
   // divided step) in the first
@@ -781,7 +812,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
           if (!in_command(c, l[i], j + i)) continue;
           const u64 w[1] = {rule.weight(l[i])}, s = (c.hi - token_ord(order_key(l[i]), j + i)) >> c.shift;
           const int b[1] = {static_cast<int>(min(s, (u64)(kBins - 1)))};
-          count_in(w, b);
+          const bool counts[1] = {w[0] != 0};
+          count_in(w, b, counts, std::true_type());
         }
       });
       collect(list, reinterpret_cast<uint32_t *>(list + kBins), 1);
@@ -995,7 +1027,7 @@ __global__ void __launch_bounds__(kValueThreads, 2) k_sample_values(const RowArg
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x / ctas, j0 = rank * p.slice, n = max(0, min(p.slice, a.vocab - j0));
   cluster.barrier_arrive();
-  if (tid < kExpTable) sh.tab[tid] = exp2(-tid / static_cast<double>(kExpTable));
+  if (tid < kExpTable) sh.tab[tid] = exp2(p.scale - tid * (1.0 / kExpTable));
   if (tid < 3) sh.tiny_mass[tid] = sh.tiny_above[tid] = 0;
   for (int i = tid; i < kPlaces; i += kValueThreads) count[i] = 0;
   serve_wait();
@@ -1074,7 +1106,7 @@ __global__ void __launch_bounds__(kValueThreads, 2) k_sample_values(const RowArg
   }
   RowRule rule;
   rule.set(high, temp, p.scale, sh.tab);
-  const double min_share = ldexp(static_cast<double>(min_p), p.scale);
+  const double min_share = static_cast<double>(min_p) * static_cast<double>(1ull << p.scale);
   // the span's least magnitude
   const float far = fmaxf(fabsf(high), greedy ? 0.0f : fabsf(fmaxf(low, high - 36.0f * temp)));
   const int least = min(max(static_cast<int>(__float_as_uint(far) >> 16) + 1 - kVals, 1), 0x7f81 - kVals);
