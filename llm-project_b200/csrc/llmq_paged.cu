@@ -313,8 +313,8 @@ cudaError_t launch_attend(AttendArgs p, int sms, cudaStream_t st) {
         std::max(1LL, std::min<long long>({tiles, (long long)sms * Sh::kPerSm, (long long)kAttendMaxCtas})));
     e = serve_launch(k_attend<Core, HDP>, dim3(ctas), dim3(kAttendThreads), Sh::kSmem, st, p);
     if (e == cudaSuccess && ctas > 1)
-      e = serve_launch(k_attend_join<typename Core::Row>, dim3(ctas, std::min(group, (int)Core::kBlock)), dim3(128), 0,
-                       st, p, ctas, (int)Core::kBlock);
+      e = serve_launch(k_attend_join<typename Core::Row>, dim3(ctas), dim3(kJoinThreads), 0, st, p, ctas,
+                       (int)Core::kBlock);
   }
   return e;
 }
@@ -445,6 +445,11 @@ extern "C" LLMQ_API int llmq_paged_attention(const LlmqPagedKV *kv, const LlmqPa
   p.kv = *kv;
   p.a = *a;
   p.scale_log2 = (a->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(kv->head_dim)) : a->scale) * 1.44269504088896341f;
+  const long long e_pool = static_cast<long long>(serve_bytes(kv->dtype));
+  p.page_bytes = kv->page_stride * e_pool;
+  p.token_bytes = kv->token_stride * e_pool;
+  p.head_bytes = kv->head_stride * e_pool;
+  set_division(p);
   int sms = 0;
   c.launched(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device));
   if (c.rc != LLMQ_OK) return c.rc;

@@ -34,7 +34,22 @@ struct AttendArgs {
   int row0, rows;      // the rows of this launch
   int blocks;          // blocks of heads a KV head
   float scale_log2;    // scale * log2(e)
+  // position / page_size, for positions below 2^31: mulhi(position, div_mul) >> div_shift
+  uint32_t div_mul;
+  int div_shift;       // below 0: page_size 1
+  long long page_bytes, token_bytes, head_bytes;  // the pool's strides
 };
+
+inline void set_division(AttendArgs &p) {
+  const uint32_t d = static_cast<uint32_t>(p.kv.page_size);
+  int l = 0;
+  while ((1u << l) < d) ++l;  // 2^(l - 1) < d <= 2^l
+  p.div_shift = l - 1;
+  p.div_mul = l ? static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d) : 0;
+}
+__device__ __forceinline__ int page_of(const AttendArgs &p, int pos) {
+  return p.div_shift < 0 ? pos : static_cast<int>(__umulhi(static_cast<uint32_t>(pos), p.div_mul) >> p.div_shift);
+}
 
 constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = kAttendWarps * 32;
@@ -59,6 +74,9 @@ inline size_t attend_workspace(int hd) {
 // ---------------------------------------------------------------- pieces
 __device__ __forceinline__ uint32_t smem_addr(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // 16 bytes to shared memory; zeros when !valid (src is not read then).
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool valid) {
@@ -526,6 +544,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   constexpr int kRounds = (HDP / kPieces + kLpr - 1) / kLpr;              // pieces of a row a lane copies
   extern __shared__ __align__(128) char s_ring[];
   __shared__ uint32_t s_mask[kAttendWarps][kAttendStages];
+  __shared__ float s_factor[kAttendWarps][kHeadBlock], s_inv[kHeadBlock];
   __shared__ long long s_sum[kAttendWarps];
   __shared__ long long s_base;
   __shared__ int s_row;
@@ -535,7 +554,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   char *ring = s_ring + (size_t)warp * (kAttendStages * Sh::kStage + Core::kSide);
   char *side = ring + kAttendStages * Sh::kStage;
   // dims past head_dim stay zero
-  for (int i = lane * 16; i < kAttendStages * Sh::kStage; i += 512) *reinterpret_cast<int4 *>(ring + i) = make_int4(0, 0, 0, 0);
+  if (hd < HDP) for (int i = lane * 16; i < kAttendStages * Sh::kStage; i += 512) *reinterpret_cast<int4 *>(ring + i) = make_int4(0, 0, 0, 0);
   serve_wait();
   serve_dependents();
 
@@ -567,7 +586,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   if (before * per_row <= x0 && x0 < (before + mine) * per_row) {
     int ignored = 0;
     for (int r = ra; r < rb; ++r) {
-      const int n = row_span(p, r, Sh::kTile, &ignored).tiles;
+      const int n = each == 1 ? static_cast<int>(mine) : row_span(p, r, Sh::kTile, &ignored).tiles;
       if (x0 < (before + n) * per_row) {
         s_row = r;
         s_base = before;
@@ -576,21 +595,25 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
       before += n;
     }
   }
-  // rows without positions
-  for (int r = p.row0 + blockIdx.x; r < p.row0 + p.rows; r += gridDim.x) {
-    int ignored = 0;
-    if (row_span(p, r, Sh::kTile, &ignored).tiles == 0) {
-      for (int e = tid; e < a.n_heads * hd; e += kAttendThreads)
-        static_cast<T *>(a.out)[r * a.out_stride + e] = from_f32<T>(0.0f);
-      for (int h = tid; h < a.n_heads && a.lse; h += kAttendThreads) a.lse[(size_t)r * a.n_heads + h] = -INFINITY;
-    }
-  }
   JoinHeader *headers = static_cast<JoinHeader *>(a.workspace);
   float *partials = reinterpret_cast<float *>(headers + gridDim.x);
   const size_t psize = attend_partial_floats(hd);
   __syncthreads();
   if (tid == 0) headers[blockIdx.x].row = -1;
-  if (x0 >= x1) return;
+  auto empty_rows = [&]() {
+    for (int r = p.row0 + blockIdx.x; r < p.row0 + p.rows; r += gridDim.x) {
+      int ignored = 0;
+      if (row_span(p, r, Sh::kTile, &ignored).tiles == 0) {
+        for (int e = tid; e < a.n_heads * hd; e += kAttendThreads)
+          static_cast<T *>(a.out)[r * a.out_stride + e] = from_f32<T>(0.0f);
+        for (int h = tid; h < a.n_heads && a.lse; h += kAttendThreads) a.lse[(size_t)r * a.n_heads + h] = -INFINITY;
+      }
+    }
+  };
+  if (x0 >= x1) {
+    empty_rows();
+    return;
+  }
 
   Cursor in;  // the next slice to fetch
   in.row = s_row;
@@ -619,48 +642,88 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
       c.span = row_span(p, c.row, Sh::kTile, &ignored);
     } while (c.span.tiles == 0);
   };
-  // lane < kSlice: the page of its key of the slice `in` points at (-1: none)
-  auto find_page = [&]() -> int {
-    const int pos = (in.span.t0 + in.tile) * Sh::kTile + warp * kSlice + lane;
-    return lane < kSlice && pos >= in.span.n0 && pos < in.span.n ? a.table[in.span.seq * a.table_stride + pos / kv.page_size]
-                                                                  : -1;
+  // Keys are looked up by runs of 8, which a page of a multiple of 8 positions does not
+  // split: a lane each, the next slice's while this one's copies are issued.  Other
+  // page sizes take a lookup a key.
+  const bool runs = kv.page_size % 8 == 0;
+  const int lookups = runs ? kSlice / 8 : kSlice, run = runs ? 8 : 1;
+  int page = -1, within = 0;  // of the lane's run: its page, the first key's place in it
+  bool asked = false;
+  auto find_page = [&]() {
+    const int pos = (in.span.t0 + in.tile) * Sh::kTile + warp * kSlice + lane * run;
+    page = -1;
+    asked = false;
+    if (lane < lookups && pos + run > in.span.n0 && pos < in.span.n) {
+      const int i = page_of(p, pos);
+      within = pos - i * kv.page_size;
+      page = a.table[in.span.seq * a.table_stride + i];  // looked at in the next fetch: no wait here
+      asked = true;
+    }
   };
   long long left = x1 - x0;  // slices to fetch
-  int page = find_page(), put = 0;
+  int put = 0;
+  find_page();
+  constexpr int kRows = 32 / kLpr;  // rows a round of copies covers
   const int piece = lane % kLpr;
+  const bool copies = piece * kPieces < hd;
+  const long long lane_bytes = (lane / kLpr) * p.token_bytes + piece * 16, round_bytes = kRows * p.token_bytes;
+  const long long to_v = static_cast<const char *>(kv.v) - static_cast<const char *>(kv.k);
   auto fetch = [&]() {
     if (left > 0) {
-      const int pos = (in.span.t0 + in.tile) * Sh::kTile + warp * kSlice + lane;
-      const bool asked = lane < kSlice && pos >= in.span.n0 && pos < in.span.n;
-      const bool good = asked && page >= 0 && page < kv.n_pages;
+      const int base = (in.span.t0 + in.tile) * Sh::kTile + warp * kSlice;
+      // keys [n0, n) of the slice, less those without a page
+      const int lo = min(max(in.span.n0 - base, 0), kSlice), hi = min(max(in.span.n - base, 0), kSlice);
+      uint32_t mask = (0xffffffffu >> 1 >> (31 - hi)) & ~((1u << lo) - 1u);
+      const bool good = asked && static_cast<unsigned>(page) < static_cast<unsigned>(kv.n_pages);
       if (asked && !good) flags |= LLMQ_PAGED_BAD_PAGE;
-      const long long off = good ? page * kv.page_stride + (pos % kv.page_size) * kv.token_stride : 0;
-      const uint32_t mask = __ballot_sync(0xffffffffu, good);
+      uint32_t have = __ballot_sync(0xffffffffu, good);
+      if (runs) have = (have & 1u ? 0xffu : 0u) | (have & 2u ? 0xff00u : 0u);
+      mask &= have;
       if (lane == 0) s_mask[warp][put] = mask;
-      const KT *kb = static_cast<const KT *>(kv.k) + in.kvh * kv.head_stride;
-      const KT *vb = static_cast<const KT *>(kv.v) + in.kvh * kv.head_stride;
-      const uint32_t dst = smem_addr(ring + put * Sh::kStage);
       if (mask) {
+        const long long off = good ? page * p.page_bytes + within * p.token_bytes : 0;
+        const char *kb = static_cast<const char *>(kv.k) + in.kvh * p.head_bytes;
+        const uint32_t dst = smem_addr(ring + put * Sh::kStage) + (lane / kLpr) * Core::kPitch + piece * 16;
+        auto copy_row = [&](uint32_t d, const char *src, bool all, bool ok) {
+          if (!copies) return;
 #pragma unroll
-        for (int it = 0; it < kSlice * kLpr / 32; ++it) {
-          const int row = it * (32 / kLpr) + lane / kLpr;
-          const long long ro = __shfl_sync(0xffffffffu, off, row);
-          const bool ok = (mask >> row) & 1u;
-#pragma unroll
-          for (int i = 0; i < kRounds; ++i) {
-            const int e = (piece + i * kLpr) * kPieces;
-            if (e < hd) {
-              const uint32_t d = dst + row * Core::kPitch + e * (int)sizeof(KT);
-              copy16(d, kb + ro + e, ok);
-              copy16(d + kSlice * Core::kPitch, vb + ro + e, ok);
+          for (int i = 0; i < kRounds; ++i)
+            if (i == 0 || (piece + i * kLpr) * kPieces < hd) {
+              const char *k = src + i * kLpr * 16;
+              if (all) {
+                copy16(d + i * kLpr * 16, k);
+                copy16(d + i * kLpr * 16 + kSlice * Core::kPitch, k + to_v);
+              } else {
+                copy16(d + i * kLpr * 16, k, ok);
+                copy16(d + i * kLpr * 16 + kSlice * Core::kPitch, k + to_v, ok);
+              }
             }
+        };
+        if (runs) {
+#pragma unroll
+          for (int g = 0; g < kSlice / 8; ++g) {
+            const char *src = kb + __shfl_sync(0xffffffffu, off, g) + lane_bytes;
+            const bool all = ((mask >> (8 * g)) & 0xffu) == 0xffu;
+#pragma unroll
+            for (int it = 0; it < 8 / kRows; ++it) {
+              const int row = 8 * g + it * kRows;
+              copy_row(dst + row * Core::kPitch, src, all, (mask >> (row + lane / kLpr)) & 1u);
+              src += round_bytes;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int it = 0; it < kSlice / kRows; ++it) {
+            const int row = it * kRows + lane / kLpr;
+            const char *src = kb + __shfl_sync(0xffffffffu, off, row) + piece * 16;
+            copy_row(dst + it * kRows * Core::kPitch, src, false, (mask >> row) & 1u);
           }
         }
       }
       put = put + 1 == kAttendStages ? 0 : put + 1;
       if (--left > 0) {
         advance(in);
-        page = find_page();
+        find_page();
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -672,6 +735,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   int get = 0;
 #pragma unroll
   for (int i = 0; i < kAttendStages - 1; ++i) fetch();
+  empty_rows();
   for (long long x = x0; x < x1; ++x) {
     const int h0 = at.kvh * group + at.block * Core::kBlock;
     const int nh = min(Core::kBlock, group - at.block * Core::kBlock);
@@ -696,33 +760,55 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
       };
       const bool out_now = ends && whole;
       float *part = partials + (2 * (size_t)blockIdx.x + (whole ? 1 : 0)) * psize;
-      for (int h = 0; h < nh; ++h) {
-        float mx = -INFINITY, sum = 0.0f, f[kAttendWarps];
+      if (tid < kHeadBlock) {  // a thread a head: the warps' factors
+        const int h = tid;
+        float mx = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kAttendWarps; ++w) mx = fmaxf(mx, of(w).m(h));
+        for (int w = 0; w < kAttendWarps; ++w) mx = h < nh ? fmaxf(mx, of(w).m(h)) : mx;
         const float ref = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
         for (int w = 0; w < kAttendWarps; ++w) {
-          f[w] = exp2_approx(of(w).m(h) - ref);
-          sum += of(w).l(h) * f[w];
+          const float f = h < nh ? exp2_approx(of(w).m(h) - ref) : 0.0f;
+          sum += h < nh ? of(w).l(h) * f : 0.0f;
+          s_factor[w][h] = f;
         }
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-        for (int d = tid; d < hd; d += kAttendThreads) {
-          float v = 0.0f;
-#pragma unroll
-          for (int w = 0; w < kAttendWarps; ++w) v += of(w).o(h, d) * f[w];
-          if (out_now)
-            static_cast<T *>(a.out)[at.row * a.out_stride + (size_t)(h0 + h) * hd + d] = from_f32<T>(v * inv);
-          else
-            part[2 * kHeadBlock + h * hd + d] = v;
-        }
-        if (tid == 0) {
+        s_inv[h] = out_now ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
+        if (h < nh) {
           if (!out_now) {
             part[h] = mx;
             part[kHeadBlock + h] = sum;
           } else if (a.lse) {
             a.lse[(size_t)at.row * a.n_heads + h0 + h] = sum > 0.0f ? (mx + log2f(sum)) * 0.693147180559945309f : -INFINITY;
           }
+        }
+      }
+      __syncthreads();
+      const bool out16 = out_now && (reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0) && a.out_stride % 4 == 0;
+#pragma unroll 2
+      for (int e = tid; e < nh * (hd / 4); e += kAttendThreads) {
+        const int h = e / (hd / 4), d = 4 * (e - h * (hd / 4));
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kAttendWarps; ++w) {
+          const float f = s_factor[w][h];
+          const float4 x = *reinterpret_cast<const float4 *>(&of(w).o(h, d));
+          v.x = fmaf(x.x, f, v.x);
+          v.y = fmaf(x.y, f, v.y);
+          v.z = fmaf(x.z, f, v.z);
+          v.w = fmaf(x.w, f, v.w);
+        }
+        const float inv = s_inv[h];
+        if (out_now) {
+          T *o = static_cast<T *>(a.out) + at.row * a.out_stride + (size_t)(h0 + h) * hd + d;
+          const Pack<T, 4> y{{from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv), from_f32<T>(v.w * inv)}};
+          if (out16) {
+            *reinterpret_cast<Pack<T, 4> *>(o) = y;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = y.v[i];
+          }
+        } else {
+          *reinterpret_cast<float4 *>(part + 2 * kHeadBlock + h * hd + d) = v;
         }
       }
       if (!whole && tid == 0) {
@@ -741,7 +827,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
       }
       __syncthreads();
       // dims past head_dim of the stage: zero again
-      for (int i = lane * 16; i < Sh::kStage; i += 512)
+      if (hd < HDP) for (int i = lane * 16; i < Sh::kStage; i += 512)
         *reinterpret_cast<int4 *>(ring + get * Sh::kStage + i) = make_int4(0, 0, 0, 0);
       fresh = whole = true;
     }
@@ -753,37 +839,80 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   if (flags && a.status) atomicOr(a.status, flags);
 }
 
-// Joins the partial results of a head that CTAs first .. last share: block
-// (c, h) the head of header c, one thread a dim.
+// Joins the partial results of the heads that CTAs first .. last of a header share:
+// one block a header, a thread four dims of a head and every kGroups-th partial result.
+constexpr int kJoinThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(128) k_attend_join(const AttendArgs p, int ctas, int head_block) {
+__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendArgs p, int ctas, int head_block) {
+  __shared__ float s_f[kAttendMaxCtas][kHeadBlock];  // factors of the partial results
+  __shared__ float4 s_v[kJoinThreads];
+  __shared__ float s_inv[kHeadBlock];
   serve_wait();
   serve_dependents();
   const LlmqPagedAttention &a = p.a;
   const JoinHeader *headers = static_cast<const JoinHeader *>(a.workspace);
-  const JoinHeader hd_ = headers[blockIdx.x];
-  if (hd_.row < 0) return;
-  const int hd = p.kv.head_dim, group = a.n_heads / p.kv.n_kv, h = blockIdx.y;
-  if (hd_.block * head_block + h >= group) return;
-  const float *partials = reinterpret_cast<const float *>(headers + ctas);
+  const JoinHeader at = headers[blockIdx.x];
+  if (at.row < 0) return;
+  const int hd = p.kv.head_dim, group = a.n_heads / p.kv.n_kv, nh = min(head_block, group - at.block * head_block);
+  const int n = at.last - at.first + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t psize = attend_partial_floats(hd);
   // the first CTA has it as the end of its share, the others as the beginning
-  auto of = [&](int c) { return partials + (2 * (size_t)c + (c == hd_.first ? 1 : 0)) * psize; };
-  float mx = -INFINITY;
-  for (int c = hd_.first; c <= hd_.last; ++c) mx = fmaxf(mx, of(c)[h]);
-  const float ref = mx == -INFINITY ? 0.0f : mx;
-  float sum = 0.0f;
-  for (int c = hd_.first; c <= hd_.last; ++c) sum += of(c)[kHeadBlock + h] * exp2_approx(of(c)[h] - ref);
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  const int head = hd_.kvh * group + hd_.block * head_block + h;
-  for (int d = threadIdx.x; d < hd; d += 128) {
-    float v = 0.0f;
-#pragma unroll 8
-    for (int c = hd_.first; c <= hd_.last; ++c) v += of(c)[2 * kHeadBlock + h * hd + d] * exp2_approx(of(c)[h] - ref);
-    static_cast<T *>(a.out)[hd_.row * a.out_stride + (size_t)head * hd + d] = from_f32<T>(v * inv);
+  const float *partials = reinterpret_cast<const float *>(headers + ctas) + 2 * (size_t)at.first * psize;
+  auto of = [&](int c) { return partials + (2 * (size_t)c + (c == 0 ? 1 : 0)) * psize; };
+  const int h0 = at.kvh * group + at.block * head_block;
+  if (warp < nh) {  // a warp a head
+    const int h = warp;
+    float mx = -INFINITY, sum = 0.0f;
+    for (int c = lane; c < n; c += 32) mx = fmaxf(mx, of(c)[h]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    for (int c = lane; c < n; c += 32) {
+      const float f = exp2_approx(of(c)[h] - ref);
+      sum += of(c)[kHeadBlock + h] * f;
+      s_f[c][h] = f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      s_inv[h] = sum > 0.0f ? 1.0f / sum : 0.0f;
+      if (a.lse) a.lse[(size_t)at.row * a.n_heads + h0 + h] = sum > 0.0f ? (mx + log2f(sum)) * 0.693147180559945309f : -INFINITY;
+    }
   }
-  if (threadIdx.x == 0 && a.lse)
-    a.lse[(size_t)hd_.row * a.n_heads + head] = sum > 0.0f ? (mx + log2f(sum)) * 0.693147180559945309f : -INFINITY;
+  __syncthreads();
+  const int pieces = nh * (hd / 4);  // at most 512
+  int groups = 1;
+  while (2 * groups * pieces <= kJoinThreads && groups < n) groups *= 2;
+  const int g = tid / pieces, e = tid - g * pieces, h = e / (hd / 4), d = 4 * (e - h * (hd / 4));
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (g < groups) {
+#pragma unroll 8
+    for (int c = g; c < n; c += groups) {
+      const float4 x = *reinterpret_cast<const float4 *>(of(c) + 2 * kHeadBlock + h * hd + d);
+      const float f = s_f[c][h];
+      v.x = fmaf(x.x, f, v.x);
+      v.y = fmaf(x.y, f, v.y);
+      v.z = fmaf(x.z, f, v.z);
+      v.w = fmaf(x.w, f, v.w);
+    }
+    s_v[tid] = v;
+  }
+  __syncthreads();
+  if (g == 0) {
+    for (int q = 1; q < groups; ++q) {
+      const float4 x = s_v[q * pieces + e];
+      v.x += x.x;
+      v.y += x.y;
+      v.z += x.z;
+      v.w += x.w;
+    }
+    const float inv = s_inv[h];
+    T *o = static_cast<T *>(a.out) + at.row * a.out_stride + (size_t)(h0 + h) * hd + d;
+    o[0] = from_f32<T>(v.x * inv);
+    o[1] = from_f32<T>(v.y * inv);
+    o[2] = from_f32<T>(v.z * inv);
+    o[3] = from_f32<T>(v.w * inv);
+  }
 }
 
 }  // namespace llmq
