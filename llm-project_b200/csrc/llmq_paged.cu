@@ -313,8 +313,8 @@ cudaError_t launch_attend(AttendArgs p, int sms, cudaStream_t st) {
         std::max(1LL, std::min<long long>({tiles, (long long)sms * Sh::kPerSm, (long long)kAttendMaxCtas})));
     e = serve_launch(k_attend<Core, HDP>, dim3(ctas), dim3(kAttendThreads), Sh::kSmem, st, p);
     if (e == cudaSuccess && ctas > 1)
-      e = serve_launch(k_attend_join<typename Core::Row>, dim3(ctas), dim3(kJoinThreads), 0, st, p, ctas,
-                       (int)Core::kBlock);
+      e = serve_launch(k_attend_join<typename Core::Row>, dim3(ctas, std::min(group, (int)Core::kBlock)),
+                       dim3(kJoinThreads), 0, st, p, ctas, (int)Core::kBlock);
   }
   return e;
 }

@@ -563,7 +563,12 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   const int ra = p.row0 + min(p.rows, tid * each), rb = p.row0 + min(p.rows, (tid + 1) * each);
   int flags = 0;
   long long mine = 0;
-  for (int r = ra; r < rb; ++r) mine += row_span(p, r, Sh::kTile, &flags).tiles;
+  bool empty = false;
+  for (int r = ra; r < rb; ++r) {
+    const int n = row_span(p, r, Sh::kTile, &flags).tiles;
+    mine += n;
+    empty |= n == 0;
+  }
   if (blockIdx.x == 0 && flags && a.status) atomicOr(a.status, flags);
   flags = 0;
   long long incl = mine;
@@ -573,7 +578,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
     if (lane >= o) incl += u;
   }
   if (lane == 31) s_sum[warp] = incl;
-  __syncthreads();
+  empty = __syncthreads_or(empty);
   long long total = 0, before = incl - mine;
   for (int w = 0; w < kAttendWarps; ++w) {
     if (w < warp) before += s_sum[w];
@@ -601,6 +606,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   __syncthreads();
   if (tid == 0) headers[blockIdx.x].row = -1;
   auto empty_rows = [&]() {
+    if (!empty) return;
     for (int r = p.row0 + blockIdx.x; r < p.row0 + p.rows; r += gridDim.x) {
       int ignored = 0;
       if (row_span(p, r, Sh::kTile, &ignored).tiles == 0) {
@@ -663,6 +669,15 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   long long left = x1 - x0;  // slices to fetch
   int put = 0;
   find_page();
+  const int group = a.n_heads / kv.n_kv;
+  Core core;
+  auto load_q = [&](const Cursor &c) {
+    const int h0 = c.kvh * group + c.block * Core::kBlock;
+    core.load_q(static_cast<const T *>(a.q) + c.row * a.q_stride + (size_t)h0 * hd, min(Core::kBlock, group - c.block * Core::kBlock),
+                hd, p.scale_log2);
+  };
+  load_q(at);  // on its way with the lookup
+  core.reset();
   constexpr int kRows = 32 / kLpr;  // rows a round of copies covers
   const int piece = lane % kLpr;
   const bool copies = piece * kPieces < hd;
@@ -729,9 +744,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  const int group = a.n_heads / kv.n_kv;
-  Core core;
-  bool fresh = true, whole = at.tile == 0;  // whole: the share has this head from its first tile
+  bool fresh = false, whole = at.tile == 0;  // whole: the share has this head from its first tile
   int get = 0;
 #pragma unroll
   for (int i = 0; i < kAttendStages - 1; ++i) fetch();
@@ -741,7 +754,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
     const int nh = min(Core::kBlock, group - at.block * Core::kBlock);
     if (fresh) {
       core.reset();
-      core.load_q(static_cast<const T *>(a.q) + at.row * a.q_stride + (size_t)h0 * hd, nh, hd, p.scale_log2);
+      load_q(at);
       fresh = false;
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(kAttendStages - 2) : "memory");
@@ -839,57 +852,63 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   if (flags && a.status) atomicOr(a.status, flags);
 }
 
-// Joins the partial results of the heads that CTAs first .. last of a header share:
-// one block a header, a thread four dims of a head and every kGroups-th partial result.
-constexpr int kJoinThreads = 512;
+// Joins the partial results of a head that CTAs first .. last of a header share:
+// block (header, head of its block), a thread four dims of every kth partial result, so
+// that a long row's few dozen are read in one or two rounds of loads.
+constexpr int kJoinThreads = 128;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendArgs p, int ctas, int head_block) {
-  __shared__ float s_f[kAttendMaxCtas][kHeadBlock];  // factors of the partial results
+  __shared__ float s_f[kAttendMaxCtas];  // factors of the partial results
   __shared__ float4 s_v[kJoinThreads];
-  __shared__ float s_inv[kHeadBlock];
+  __shared__ float s_red[2][kJoinThreads / 32];
   serve_wait();
   serve_dependents();
   const LlmqPagedAttention &a = p.a;
   const JoinHeader *headers = static_cast<const JoinHeader *>(a.workspace);
   const JoinHeader at = headers[blockIdx.x];
-  if (at.row < 0) return;
-  const int hd = p.kv.head_dim, group = a.n_heads / p.kv.n_kv, nh = min(head_block, group - at.block * head_block);
+  const int hd = p.kv.head_dim, group = a.n_heads / p.kv.n_kv, h = blockIdx.y;
+  if (at.row < 0 || at.block * head_block + h >= group) return;
   const int n = at.last - at.first + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t psize = attend_partial_floats(hd);
   // the first CTA has it as the end of its share, the others as the beginning
   const float *partials = reinterpret_cast<const float *>(headers + ctas) + 2 * (size_t)at.first * psize;
   auto of = [&](int c) { return partials + (2 * (size_t)c + (c == 0 ? 1 : 0)) * psize; };
-  const int h0 = at.kvh * group + at.block * head_block;
-  if (warp < nh) {  // a warp a head
-    const int h = warp;
-    float mx = -INFINITY, sum = 0.0f;
-    for (int c = lane; c < n; c += 32) mx = fmaxf(mx, of(c)[h]);
+  constexpr int kMine = (kAttendMaxCtas + kJoinThreads - 1) / kJoinThreads;
+  float m[kMine], l[kMine], mx = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float ref = mx == -INFINITY ? 0.0f : mx;
-    for (int c = lane; c < n; c += 32) {
-      const float f = exp2_approx(of(c)[h] - ref);
-      sum += of(c)[kHeadBlock + h] * f;
-      s_f[c][h] = f;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-      s_inv[h] = sum > 0.0f ? 1.0f / sum : 0.0f;
-      if (a.lse) a.lse[(size_t)at.row * a.n_heads + h0 + h] = sum > 0.0f ? (mx + log2f(sum)) * 0.693147180559945309f : -INFINITY;
-    }
+  for (int i = 0; i < kMine; ++i) {
+    const int c = tid + i * kJoinThreads;
+    m[i] = c < n ? of(c)[h] : -INFINITY;
+    l[i] = c < n ? of(c)[kHeadBlock + h] : 0.0f;
+    mx = fmaxf(mx, m[i]);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) s_red[0][warp] = mx;
   __syncthreads();
-  const int pieces = nh * (hd / 4);  // at most 512
-  int groups = 1;
-  while (2 * groups * pieces <= kJoinThreads && groups < n) groups *= 2;
-  const int g = tid / pieces, e = tid - g * pieces, h = e / (hd / 4), d = 4 * (e - h * (hd / 4));
+  for (int w = 0; w < kJoinThreads / 32; ++w) mx = fmaxf(mx, s_red[0][w]);
+  const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int c = tid + i * kJoinThreads;
+    const float f = exp2_approx(m[i] - ref);
+    sum += l[i] * f;
+    if (c < n) s_f[c] = f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) s_red[1][warp] = sum;
+  __syncthreads();
+  sum = 0.0f;
+  for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_red[1][w];
+  const int pieces = hd / 4;  // at most 64
+  const int groups = kJoinThreads / pieces, g = tid / pieces, d = 4 * (tid - g * pieces);
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (g < groups) {
 #pragma unroll 8
     for (int c = g; c < n; c += groups) {
       const float4 x = *reinterpret_cast<const float4 *>(of(c) + 2 * kHeadBlock + h * hd + d);
-      const float f = s_f[c][h];
+      const float f = s_f[c];
       v.x = fmaf(x.x, f, v.x);
       v.y = fmaf(x.y, f, v.y);
       v.z = fmaf(x.z, f, v.z);
@@ -898,21 +917,24 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendArgs p
     s_v[tid] = v;
   }
   __syncthreads();
+  const int head = at.kvh * group + at.block * head_block + h;
   if (g == 0) {
-    for (int q = 1; q < groups; ++q) {
-      const float4 x = s_v[q * pieces + e];
+    for (int q = 1; q < min(groups, n); ++q) {
+      const float4 x = s_v[q * pieces + tid];
       v.x += x.x;
       v.y += x.y;
       v.z += x.z;
       v.w += x.w;
     }
-    const float inv = s_inv[h];
-    T *o = static_cast<T *>(a.out) + at.row * a.out_stride + (size_t)(h0 + h) * hd + d;
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    T *o = static_cast<T *>(a.out) + at.row * a.out_stride + (size_t)head * hd + d;
     o[0] = from_f32<T>(v.x * inv);
     o[1] = from_f32<T>(v.y * inv);
     o[2] = from_f32<T>(v.z * inv);
     o[3] = from_f32<T>(v.w * inv);
   }
+  if (tid == 0 && a.lse)
+    a.lse[(size_t)at.row * a.n_heads + head] = sum > 0.0f ? (mx + log2f(sum)) * 0.693147180559945309f : -INFINITY;
 }
 
 }  // namespace llmq
