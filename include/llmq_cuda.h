@@ -687,6 +687,54 @@ typedef struct {
 } LlmqSampleRows;
 int llmq_sample_rows(const LlmqSampleRows *a, void *stream);
 
+/* ---- batches of a model with these operators ---- */
+
+/* Settings of llmq_sample_rows for each sequence, in host memory; a null array is
+ * off (temperature: 1).  u is needed. */
+typedef struct {
+  const float *temperature;
+  const int *top_k;
+  const float *top_p, *min_p;
+  const float *u;
+} LlmqSampling;
+
+/* As q_llama_decode_batch_argmax, with each next token drawn by llmq_sample_rows
+ * from its row's logits: ids[b] from s->u[b] and the settings of sequence b.
+ * Not under tensor parallelism.  Returns 0 or an error code. */
+int q_llama_decode_batch_sample(const QLlamaModel *m, LlamaKV **kvs, const int *tokens, int B, const LlmqSampling *s,
+                                int *ids);
+
+/* A paged cache of up to max_seqs sequences of a model: n_pages pages of
+ * page_size positions (of every layer), shared out as the sequences grow, in
+ * place of one max_seq cache a sequence.  dtype is the pages' type; sequences
+ * start empty.  head_dim must be a multiple of 8, at most 256.  Not under tensor
+ * parallelism.  NULL on error.  The cache belongs to the model: freeing the model
+ * frees it (the handle is then invalid). */
+typedef struct LlmqPagedCache LlmqPagedCache;
+LlmqPagedCache *q_llama_paged_create(const QLlamaModel *m, int n_pages, int page_size, int max_seqs, int dtype);
+void q_llama_paged_free(LlmqPagedCache *c);
+/* Positions sequence seq holds, or -1 on error; pages that no sequence holds. */
+int q_llama_paged_len(const LlmqPagedCache *c, int seq);
+int q_llama_paged_free_pages(const LlmqPagedCache *c);
+/* Empties sequence seq: its pages are free again.  Returns 0 or an error code. */
+int q_llama_paged_reset(LlmqPagedCache *c, int seq);
+
+/* One step of a batch: sequence b takes added[b] tokens (0: it sits out; 1: a
+ * decode step; more: a prompt or a piece of one), listed in `tokens` sequence
+ * after sequence.  All rows go through the layers together: llmq_paged_plan,
+ * then in each layer llmq_paged_append and llmq_paged_attention, and one
+ * llmq_sample_rows (s null: the greedy choice) for the last row of every sequence
+ * that took any.  ids[b] receives sequence b's next token (-1 if it sat out);
+ * `logits`, if given, the rows ids came from, one below the other for the
+ * sequences that took tokens, in their order.  Attention runs as documented at
+ * llmq_paged_attention: unlike q_llama_decode_batch it does not keep the
+ * reference's order of additions, so logits are near that path's, not equal bit
+ * for bit.  An error leaves the sequences as they were, except LLMQ_ERR_CUDA,
+ * after which the cache answers LLMQ_ERR_STATE until it is freed.  Returns 0 or an
+ * error code. */
+int q_llama_paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const int *tokens,
+                       const LlmqSampling *s, int *ids, Tensor *logits);
+
 #ifdef __cplusplus
 }
 #endif

@@ -748,6 +748,7 @@ struct DevModel {
   char **tpx_peers_dev = nullptr;    // the same, in device memory
   unsigned *tp_seq = nullptr;        // row-parallel products completed
   std::vector<DevKV *> kvs;
+  std::vector<LlmqPagedCache *> paged;
   // per-kernel events while llmq_step_profile records a step outside a graph
   std::vector<cudaEvent_t> *prof = nullptr;
   // multi-row passes (batched decode, prefill): grow-only scratch
@@ -777,6 +778,8 @@ void release_kv(DevKV *K) {
   delete K;
 }
 
+void release_paged(LlmqPagedCache *c);
+
 void release_model(DevModel *M) {
   int cur = -1;
   cudaGetDevice(&cur);
@@ -786,6 +789,7 @@ void release_model(DevModel *M) {
     g_kvs.erase(K->key);
     release_kv(K);
   }
+  for (LlmqPagedCache *c : M->paged) release_paged(c);
   for (auto *v : {&M->qkv, &M->wo, &M->w13, &M->w2})
     for (Mat &m : *v) free_mat(m);
   free_mat(M->lm);
@@ -1753,11 +1757,23 @@ int ensure_rows(DevModel *M, int rows, int lm_rows) {
   return 1;
 }
 
+// What a pass does differently: over a paged cache its rows' keys, values and
+// attention go through the pages; rows of the residual stream given apart skip the
+// layers; the next tokens of the lm-head's rows are drawn instead of the greedy ids.
+struct RowsHook {
+  const LlmqPagedCache *paged = nullptr;
+  int row0 = 0;                          // the pass's first row in the step
+  const float *x = nullptr;              // [rows][d_model]: no layers, the lm-head only
+  const LlmqSampleRows *sample = nullptr;  // settings (device); logits and ids are set here
+};
+int paged_attention(const LlmqPagedCache &c, DevModel *M, int layer, int row0, int rows);
+
 // One pass over `rows` rows (each one decode step of its own sequence, at its
 // own position).  All layers run for every row; the final norm, lm-head and
 // greedy id run for rows [lm0, rows) only: their ids go to ids_h and, if
 // logits_h is given, their logits (row-major, vocab per row) as well.
-int run_rows(DevCtx &c, DevModel *M, const RowDesc *rows_h, int rows, int lm0, float *logits_h, int *ids_h) {
+int run_rows(DevCtx &c, DevModel *M, const RowDesc *rows_h, int rows, int lm0, float *logits_h, int *ids_h,
+             const RowsHook &hook = RowsHook()) {
   const LlmqConfig &cfg = M->cfg;
   cudaStream_t st = M->stream;
 
@@ -1810,7 +1826,8 @@ int run_rows(DevCtx &c, DevModel *M, const RowDesc *rows_h, int rows, int lm0, f
   const int pf_rpb = pf_rows_per_block(group);
   const size_t pf_sm = pf_scores_smem(hd);
   const int attn_threads = (group * hd / 2 + 31) / 32 * 32;  // k_rows_pv: two output dims per thread
-  if (hd % 4 != 0 || group > kAttnMaxGroup || attn_threads > 1024 || pv_sm + 4096 > (size_t)g_smem_optin) {
+  if (!hook.paged && !hook.x &&
+      (hd % 4 != 0 || group > kAttnMaxGroup || attn_threads > 1024 || pv_sm + 4096 > (size_t)g_smem_optin)) {
     llmq_set_error(LLMQ_ERR_ARG, "libllmq_cuda: batched attention needs head_dim %% 4 == 0, group <= %d, "
                    "group*head_dim <= 1024 and max_seq %d short enough for shared memory", kAttnMaxGroup,
                    cfg.max_seq);
@@ -1859,18 +1876,26 @@ int run_rows(DevCtx &c, DevModel *M, const RowDesc *rows_h, int rows, int lm0, f
     NK(g_nccl.AllReduce(t.acc, t.acc, (size_t)rows * m.Npad, ncclInt32, ncclSum, g_tp.comm, st));
     return launch_tc_epilogue(t, st);
   };
-  for (int l = 0; l < cfg.n_layers; ++l) {
+  for (int l = 0; l < cfg.n_layers && !hook.x; ++l) {
     CK(norm(l == 0 ? nullptr : R.x, M->attn_norm[l], M->qkv[l], rows));
     if (!gemm(M->qkv[l], rows, TC_BIAS, M->bias_qkv[l], R.qkv, qd + 2 * kvd, nullptr)) return 0;
     aa.layer = l;
-    CK(launch_pdl(k_rows_append, dim3(rows), dim3(256), 0, st, aa));
-    if (pf_tiled)  // a prefill: each key chunk staged once per block of rows
+    if (hook.paged) {
+      if (!paged_attention(*hook.paged, M, l, hook.row0, rows)) return 0;
+    } else {
+      CK(launch_pdl(k_rows_append, dim3(rows), dim3(256), 0, st, aa));
+    }
+    if (hook.paged) {
+      // done
+    } else if (pf_tiled)  // a prefill: each key chunk staged once per block of rows
       CK(launch_pdl(k_pf_scores, dim3((cfg.max_seq + kPfVecs - 1) / kPfVecs, cfg.n_kv, (rows + pf_rpb - 1) / pf_rpb),
                     dim3(256), pf_sm, st, aa, rows));
     else
       CK(launch_pdl(k_rows_scores, dim3((cfg.max_seq + kRowScoreKeys - 1) / kRowScoreKeys, cfg.n_kv, rows),
                     dim3(kRowScoreThreads), sc_sm, st, aa));
-    if (pf_tiled && hd == 128 && (size_t)group * ((cfg.max_seq + 3) & ~3) * 4 + 4096 <= (size_t)g_smem_optin) {
+    if (hook.paged) {
+      // done
+    } else if (pf_tiled && hd == 128 && (size_t)group * ((cfg.max_seq + 3) & ~3) * 4 + 4096 <= (size_t)g_smem_optin) {
       // softmax in place, then the row-block tiled values
       CK(launch_pdl(k_pf_softmax, dim3(rows, cfg.n_kv), dim3(256), (size_t)group * ((cfg.max_seq + 3) & ~3) * 4, st,
                     aa));
@@ -1894,11 +1919,21 @@ int run_rows(DevCtx &c, DevModel *M, const RowDesc *rows_h, int rows, int lm0, f
     }
   }
   if (lm_rows > 0) {
-    CK(norm(R.x + (size_t)lm0 * dm, M->final_norm, M->lm, lm_rows));
+    CK(norm(hook.x ? hook.x : R.x + (size_t)lm0 * dm, M->final_norm, M->lm, lm_rows));
     if (!gemm(M->lm, lm_rows, TC_LOGITS, nullptr, R.logits, cfg.vocab, R.argmax)) return 0;
     if (M->tp_world > 1)  // the first maximum over every shard's vocab slice (sampler.c:8-21)
       NK(g_nccl.AllReduce(R.argmax, R.argmax, (size_t)lm_rows, ncclUint64, ncclMax, g_tp.comm, st));
     CK(launch_pdl(k_rows_finish, dim3(1), dim3(256), 0, st, R.argmax, lm_rows, R.ids));
+    if (hook.sample) {
+      LlmqSampleRows sr = *hook.sample;
+      sr.n_rows = lm_rows;
+      sr.vocab = cfg.vocab;
+      sr.dtype = LLMQ_F32;
+      sr.logits = R.logits;
+      sr.stride = cfg.vocab;
+      sr.ids = R.ids;
+      if (llmq_sample_rows(&sr, st) != LLMQ_OK) return 0;
+    }
     CK(cudaMemcpyAsync(R.h_ids, R.ids, (size_t)lm_rows * sizeof(int), cudaMemcpyDeviceToHost, st));
     if (logits_h && M->tp_world > 1) {
       // gathered as [rank][rows][vocab slice]: each rank's block lands in its
@@ -1922,6 +1957,92 @@ int run_rows(DevCtx &c, DevModel *M, const RowDesc *rows_h, int rows, int lm0, f
     return reset_after_device_error(M, R.h_err[0]);
   }
   if (lm_rows > 0 && ids_h) std::memcpy(ids_h, R.h_ids, (size_t)lm_rows * sizeof(int));
+  return 1;
+}
+
+// Sampling settings of n sequences on the GPU, in columns.
+struct SampleColumns {
+  float *dev = nullptr;
+  size_t n = 0;
+  bool has[5] = {};
+  SampleColumns() = default;
+  SampleColumns(const SampleColumns &) = delete;
+  ~SampleColumns() { cudaFree(dev); }
+  // of the sequences listed in `which` (null: 0 .. count)
+  int fill(const LlmqSampling &s, int count, const int *which, cudaStream_t st) {
+    n = static_cast<size_t>(count);
+    std::vector<float> h(5 * n);
+    const void *src[5] = {s.temperature, s.top_k, s.top_p, s.min_p, s.u};
+    for (int c = 0; c < 5; ++c) {
+      has[c] = src[c] != nullptr;
+      for (size_t i = 0; i < n && has[c]; ++i)  // 4 bytes each, whatever they mean
+        std::memcpy(&h[c * n + i], static_cast<const char *>(src[c]) + 4 * (which ? (size_t)which[i] : i), 4);
+    }
+    CK(cudaMalloc(&dev, 5 * n * sizeof(float)));
+    CK(cudaMemcpyAsync(dev, h.data(), 5 * n * sizeof(float), cudaMemcpyHostToDevice, st));
+    CK(cudaStreamSynchronize(st));  // h ends here
+    return 1;
+  }
+  LlmqSampleRows rows(int first) const {
+    LlmqSampleRows r{};
+    r.temperature = has[0] ? dev + first : nullptr;
+    r.top_k = has[1] ? reinterpret_cast<const int *>(dev + n) + first : nullptr;
+    r.top_p = has[2] ? dev + 2 * n + first : nullptr;
+    r.min_p = has[3] ? dev + 3 * n + first : nullptr;
+    r.u = dev + 4 * n + first;
+    return r;
+  }
+};
+
+// B sequences, one token each: greedy ids, or drawn by the settings of `smp`.
+int decode_rows(const QLlamaModel *m, LlamaKV *const *kvs, const int *tokens, int B, float *logits, int *ids,
+                const LlmqSampling *smp) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (B <= 0 || !kvs || !tokens) {
+    llmq_set_error(LLMQ_ERR_ARG, "q_llama_decode_batch: bad arguments");
+    return 0;
+  }
+  DevModel *M = get_model(m);
+  if (!M) return 0;
+  DevCtx *c = get_ctx();
+  if (!c) return 0;
+  std::vector<RowDesc> rows((size_t)B);
+  for (int b = 0; b < B; ++b) {
+    const LlamaKV *kv = kvs[b];
+    DevKV *K = get_kv(M, kv);
+    if (!K || !check_step_inputs(M, kv, tokens[b], 1)) return 0;
+    for (int e = 0; e < b; ++e)
+      if (rows[e].k == K->k) {
+        llmq_set_error(LLMQ_ERR_ARG, "q_llama_decode_batch: sequence %d and %d share one KV cache", e, b);
+        return 0;
+      }
+    rows[b] = RowDesc{K->k, K->v, K->max_seq, kv->len, tokens[b], 0};
+  }
+  std::vector<int> tmp;
+  if (!ids) {
+    tmp.resize((size_t)B);
+    ids = tmp.data();
+  }
+  SampleColumns cols;
+  if (smp && !cols.fill(*smp, B, nullptr, M->stream)) return 0;
+  g_launches = 0;
+  CK(cudaEventRecord(M->ev0, M->stream));
+  for (int off = 0; off < B; off += kRowsPerPass) {
+    const int n = std::min(kRowsPerPass, B - off);
+    RowsHook hook;
+    LlmqSampleRows sr{};
+    if (smp) {
+      sr = cols.rows(off);
+      hook.sample = &sr;
+    }
+    if (!run_rows(*c, M, rows.data() + off, n, 0, logits ? logits + (size_t)off * M->vocab_full : nullptr, ids + off,
+                  hook))
+      return 0;
+  }
+  CK(cudaEventRecord(M->ev1, M->stream));
+  CK(cudaEventSynchronize(M->ev1));
+  cudaEventElapsedTime(&g_last_ms, M->ev0, M->ev1);
+  g_last_launches = g_launches;
   return 1;
 }
 
@@ -2284,44 +2405,7 @@ int llmqd_sample_row(const float *row, int V, LlmqSample *smp, int *id) {
 
 int llmqd_decode_rows(const QLlamaModel *m, LlamaKV *const *kvs, const int *tokens, int B, float *logits,
                       int *ids) {
-  std::lock_guard<std::recursive_mutex> lk(g_mu);
-  if (B <= 0 || !kvs || !tokens) {
-    llmq_set_error(LLMQ_ERR_ARG, "q_llama_decode_batch: bad arguments");
-    return 0;
-  }
-  DevModel *M = get_model(m);
-  if (!M) return 0;
-  DevCtx *c = get_ctx();
-  if (!c) return 0;
-  std::vector<RowDesc> rows((size_t)B);
-  for (int b = 0; b < B; ++b) {
-    const LlamaKV *kv = kvs[b];
-    DevKV *K = get_kv(M, kv);
-    if (!K || !check_step_inputs(M, kv, tokens[b], 1)) return 0;
-    for (int e = 0; e < b; ++e)
-      if (rows[e].k == K->k) {
-        llmq_set_error(LLMQ_ERR_ARG, "q_llama_decode_batch: sequence %d and %d share one KV cache", e, b);
-        return 0;
-      }
-    rows[b] = RowDesc{K->k, K->v, K->max_seq, kv->len, tokens[b], 0};
-  }
-  std::vector<int> tmp;
-  if (!ids) {
-    tmp.resize((size_t)B);
-    ids = tmp.data();
-  }
-  g_launches = 0;
-  CK(cudaEventRecord(M->ev0, M->stream));
-  for (int off = 0; off < B; off += kRowsPerPass) {
-    const int n = std::min(kRowsPerPass, B - off);
-    if (!run_rows(*c, M, rows.data() + off, n, 0, logits ? logits + (size_t)off * M->vocab_full : nullptr, ids + off))
-      return 0;
-  }
-  CK(cudaEventRecord(M->ev1, M->stream));
-  CK(cudaEventSynchronize(M->ev1));
-  cudaEventElapsedTime(&g_last_ms, M->ev0, M->ev1);
-  g_last_launches = g_launches;
-  return 1;
+  return decode_rows(m, kvs, tokens, B, logits, ids, nullptr);
 }
 
 int llmqd_prefill(const QLlamaModel *m, const LlamaKV *kv, const int *ids, int n, float *logits, int *next) {
@@ -3002,3 +3086,5 @@ extern "C" LLMQ_API int llmq_rmsnorm_qmatmul(const float *x, const float *gamma,
   free_mat(m);
   return rc;
 }
+
+#include "llmq_paged_model.cuh"

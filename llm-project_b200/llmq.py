@@ -110,6 +110,24 @@ class SampleRows(C.Structure):
                        (C.c_void_p, "temperature top_k top_p min_p u ids logprobs"))
 
 
+class Sampling(C.Structure):
+    _fields_ = [("temperature", c_float_p), ("top_k", c_int_p), ("top_p", c_float_p), ("min_p", c_float_p),
+                ("u", c_float_p)]
+
+
+def sampling(temperature=None, top_k=None, top_p=None, min_p=None, u=None) -> Sampling:
+    """A Sampling struct over numpy copies of the given per-sequence values."""
+    keep, s = [], Sampling()
+    for name, v, t, p in (("temperature", temperature, np.float32, c_float_p), ("top_k", top_k, np.int32, c_int_p),
+                          ("top_p", top_p, np.float32, c_float_p), ("min_p", min_p, np.float32, c_float_p),
+                          ("u", u, np.float32, c_float_p)):
+        if v is not None:
+            keep.append(np.ascontiguousarray(v, dtype=t))
+            setattr(s, name, keep[-1].ctypes.data_as(p))
+    s._keep = keep
+    return s
+
+
 def config(vocab, d_model, n_layers, n_heads, n_kv, head_dim, d_ff, max_seq, rope_base=10000.0,
            eps=1e-5) -> LlmqConfig:
     return LlmqConfig(vocab, d_model, n_layers, n_heads, n_kv, head_dim, d_ff, max_seq, rope_base, eps)
@@ -193,6 +211,15 @@ SIGNATURES = {
     "q_llama_tp_unique_id": (C.c_int, [C.c_char_p]),
     "q_llama_tp_init": (C.c_int, [C.c_int, C.c_int, C.c_char_p]),
     "q_llama_tp_shutdown": (None, []),
+    "q_llama_decode_batch_sample": (C.c_int, [C.POINTER(QLlamaModel), C.POINTER(C.POINTER(LlamaKV)), c_int_p, C.c_int,
+                                              C.POINTER(Sampling), c_int_p]),
+    "q_llama_paged_create": (C.c_void_p, [C.POINTER(QLlamaModel), C.c_int, C.c_int, C.c_int, C.c_int]),
+    "q_llama_paged_free": (None, [C.c_void_p]),
+    "q_llama_paged_len": (C.c_int, [C.c_void_p, C.c_int]),
+    "q_llama_paged_free_pages": (C.c_int, [C.c_void_p]),
+    "q_llama_paged_reset": (C.c_int, [C.c_void_p, C.c_int]),
+    "q_llama_paged_step": (C.c_int, [C.POINTER(QLlamaModel), C.c_void_p, c_int_p, c_int_p, C.POINTER(Sampling),
+                                     c_int_p, C.POINTER(Tensor)]),
     "llmq_paged_plan": (C.c_int, [C.POINTER(PagedPlan), C.c_void_p]),
     "llmq_paged_append": (C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAppend), C.c_void_p]),
     "llmq_paged_attention": (C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAttention), C.c_void_p]),
