@@ -729,9 +729,11 @@ int q_llama_paged_reset(LlmqPagedCache *c, int seq);
  * sequences that took tokens, in their order.  Attention runs as documented at
  * llmq_paged_attention: unlike q_llama_decode_batch it does not keep the
  * reference's order of additions, so logits are near that path's, not equal bit
- * for bit.  An error leaves the sequences as they were, except LLMQ_ERR_CUDA,
- * after which the cache answers LLMQ_ERR_STATE until it is freed.  Returns 0 or an
- * error code. */
+ * for bit.  A row reads its sequence's keys and values on its own: made for decode
+ * steps and short prompts; q_llama_prefill is the one that shares them among a
+ * prompt's rows.  An error leaves the sequences as they were; after one of the GPU
+ * in the middle of a step the cache answers LLMQ_ERR_STATE until it is freed.
+ * Returns 0 or an error code. */
 int q_llama_paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const int *tokens,
                        const LlmqSampling *s, int *ids, Tensor *logits);
 
