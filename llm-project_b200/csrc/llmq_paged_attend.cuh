@@ -56,6 +56,10 @@ constexpr int kAttendThreads = kAttendWarps * 32;
 constexpr int kAttendStages = 3;
 constexpr int kAttendMaxRows = 1024;  // rows of one launch
 constexpr int kHeadBlock = 8;         // query heads of a partial result
+// Units of a head beside its tiles: what joining the warps and fetching the next query
+// cost, about two tiles' time.  Ragged bf16 rows of up to 8191 positions: 204 us without,
+// 192 with one, 184 with two or three; 150 rows of up to 1000: 95, 77, 68, 69 us.
+constexpr int kLead = 2;
 
 // ------------------------------------------------------------- workspace
 // For each CTA a header (the head it must join with earlier CTAs, if any) and two
@@ -530,6 +534,7 @@ struct AttendShape {
 struct Cursor {
   RowSpan span;
   int row, kvh, block, tile;
+  long long unit;
 };
 
 template <typename Core, int HDP>
@@ -545,7 +550,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   extern __shared__ __align__(128) char s_ring[];
   __shared__ uint32_t s_mask[kAttendWarps][kAttendStages];
   __shared__ float s_factor[kAttendWarps][kHeadBlock], s_inv[kHeadBlock];
-  __shared__ long long s_sum[kAttendWarps];
+  __shared__ long long s_sum[kAttendWarps], s_rows[kAttendWarps];
   __shared__ long long s_base;
   __shared__ int s_row;
   const LlmqPagedKV &kv = p.kv;
@@ -558,40 +563,55 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   serve_wait();
   serve_dependents();
 
-  // ---- this CTA's share: tiles [x0, x1) of per_row * (tiles of all rows)
+  // ---- this CTA's share: units [x0, x1).  A head takes a unit a tile, after `lead` units
+  // for what its end costs beside its tiles (joining the warps, the next head's query)
   const int per_row = kv.n_kv * p.blocks, each = (p.rows + kAttendThreads - 1) / kAttendThreads;
   const int ra = p.row0 + min(p.rows, tid * each), rb = p.row0 + min(p.rows, (tid + 1) * each);
   int flags = 0;
-  long long mine = 0;
-  bool empty = false;
+  long long mine = 0, mine_rows = 0;
   for (int r = ra; r < rb; ++r) {
     const int n = row_span(p, r, Sh::kTile, &flags).tiles;
     mine += n;
-    empty |= n == 0;
+    mine_rows += n > 0;
   }
+  const bool empty = __syncthreads_or(mine_rows < rb - ra);  // some row has no position
   if (blockIdx.x == 0 && flags && a.status) atomicOr(a.status, flags);
   flags = 0;
-  long long incl = mine;
+  long long incl = mine, incl_rows = mine_rows;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += u;
+    const long long u = __shfl_up_sync(0xffffffffu, incl, o), v = __shfl_up_sync(0xffffffffu, incl_rows, o);
+    if (lane >= o) {
+      incl += u;
+      incl_rows += v;
+    }
   }
-  if (lane == 31) s_sum[warp] = incl;
-  empty = __syncthreads_or(empty);
-  long long total = 0, before = incl - mine;
+  if (lane == 31) {
+    s_sum[warp] = incl;
+    s_rows[warp] = incl_rows;
+  }
+  __syncthreads();
+  long long total = 0, rows_total = 0, before = incl - mine, rows_before = incl_rows - mine_rows;
   for (int w = 0; w < kAttendWarps; ++w) {
-    if (w < warp) before += s_sum[w];
+    if (w < warp) {
+      before += s_sum[w];
+      rows_before += s_rows[w];
+    }
     total += s_sum[w];
+    rows_total += s_rows[w];
   }
-  total *= per_row;
+  // with only a few tiles a CTA the tiles themselves are spread as evenly as they can be
+  const int lead = total * per_row > 4LL * gridDim.x ? kLead : 0;
+  total = (total + lead * rows_total) * per_row;
+  before += lead * rows_before;
+  mine += lead * mine_rows;
   const long long ctas = min(static_cast<long long>(gridDim.x), total);  // none has an empty share
   const bool idle = blockIdx.x >= ctas;
   const long long x0 = idle ? total : blockIdx.x * total / ctas, x1 = idle ? total : (blockIdx.x + 1) * total / ctas;
   if (before * per_row <= x0 && x0 < (before + mine) * per_row) {
     int ignored = 0;
     for (int r = ra; r < rb; ++r) {
-      const int n = each == 1 ? static_cast<int>(mine) : row_span(p, r, Sh::kTile, &ignored).tiles;
+      const int t = row_span(p, r, Sh::kTile, &ignored).tiles, n = t ? t + lead : 0;
       if (x0 < (before + n) * per_row) {
         s_row = r;
         s_base = before;
@@ -628,16 +648,23 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
     in.span = row_span(p, in.row, Sh::kTile, &ignored);
   }
   {
-    const long long rel = x0 - s_base * per_row;
-    const int pair = static_cast<int>(rel / in.span.tiles);
-    in.tile = static_cast<int>(rel - (long long)pair * in.span.tiles);
+    const long long rel = x0 - s_base * per_row, size = in.span.tiles + lead;
+    const int pair = static_cast<int>(rel / size), in_pair = static_cast<int>(rel - pair * size);
+    in.tile = max(0, in_pair - lead);
+    in.unit = x0 - in_pair + lead + in.tile;
     in.kvh = pair / p.blocks;
     in.block = pair - in.kvh * p.blocks;
   }
+  if (in.unit >= x1) {  // a share of lead units alone
+    empty_rows();
+    return;
+  }
   Cursor at = in;  // the slice to add
   auto advance = [&](Cursor &c) {
+    ++c.unit;
     if (++c.tile < c.span.tiles) return;
     c.tile = 0;
+    c.unit += lead;
     if (++c.block < p.blocks) return;
     c.block = 0;
     if (++c.kvh < kv.n_kv) return;
@@ -666,7 +693,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
       asked = true;
     }
   };
-  long long left = x1 - x0;  // slices to fetch
+  bool more = true;  // slices to fetch
   int put = 0;
   find_page();
   const int group = a.n_heads / kv.n_kv;
@@ -684,7 +711,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
   const long long lane_bytes = (lane / kLpr) * p.token_bytes + piece * 16, round_bytes = kRows * p.token_bytes;
   const long long to_v = static_cast<const char *>(kv.v) - static_cast<const char *>(kv.k);
   auto fetch = [&]() {
-    if (left > 0) {
+    if (more) {
       const int base = (in.span.t0 + in.tile) * Sh::kTile + warp * kSlice;
       // keys [n0, n) of the slice, less those without a page
       const int lo = min(max(in.span.n0 - base, 0), kSlice), hi = min(max(in.span.n - base, 0), kSlice);
@@ -736,10 +763,9 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
         }
       }
       put = put + 1 == kAttendStages ? 0 : put + 1;
-      if (--left > 0) {
-        advance(in);
-        find_page();
-      }
+      advance(in);
+      more = in.unit < x1;
+      if (more) find_page();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -749,7 +775,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
 #pragma unroll
   for (int i = 0; i < kAttendStages - 1; ++i) fetch();
   empty_rows();
-  for (long long x = x0; x < x1; ++x) {
+  while (true) {
     const int h0 = at.kvh * group + at.block * Core::kBlock;
     const int nh = min(Core::kBlock, group - at.block * Core::kBlock);
     if (fresh) {
@@ -762,7 +788,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
     const uint32_t mask = s_mask[warp][get];
     if (mask) core.add(ring + get * Sh::kStage, side, mask, p.scale_log2);
     const bool ends = at.tile + 1 == at.span.tiles;
-    if (ends || x + 1 == x1) {
+    if (ends || at.unit + 1 == x1) {
       // ---- the head, or the share's part of it, is done: join the warps
       __syncwarp();
       core.write(PartialBuf<HDP>{reinterpret_cast<float *>(ring + get * Sh::kStage)});
@@ -826,7 +852,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
       }
       if (!whole && tid == 0) {
         // this CTA begins inside the head: the second CTA of the head sees to the join
-        const long long g0 = x - at.tile, g1 = g0 + at.span.tiles;
+        const long long g0 = at.unit - at.tile, g1 = g0 + at.span.tiles;
         const long long first = ((g0 + 1) * ctas - 1) / total, last = (g1 * ctas - 1) / total;
         if (first + 1 == blockIdx.x) {
           JoinHeader h{};
@@ -846,7 +872,8 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
     }
     __syncwarp();
     get = get + 1 == kAttendStages ? 0 : get + 1;
-    if (x + 1 < x1) advance(at);
+    advance(at);
+    if (at.unit >= x1) break;
     fetch();
   }
   if (flags && a.status) atomicOr(a.status, flags);
