@@ -628,8 +628,8 @@ int llmq_paged_append(const LlmqPagedKV *kv, const LlmqPagedAppend *a, void *str
  * pools, 24 for f32 rows over bf16).  The result depends on the batch only in
  * the order of its sums.  A row without positions gives zeros and lse -infinity.
  * Positions on a page outside the pool are left out.  What the pool holds past
- * a row's length is never read into a result.  scale 0 stands for
- * 1 / sqrt(head_dim).  The workspace need not be initialised; calls that may
+ * a row's length is never read into a result.  out may not overlap q.  scale 0
+ * stands for 1 / sqrt(head_dim).  The workspace need not be initialised; calls that may
  * overlap need one each. */
 typedef struct {
   int n_rows, n_heads;

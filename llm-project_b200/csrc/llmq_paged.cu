@@ -455,7 +455,8 @@ extern "C" LLMQ_API int llmq_paged_attention(const LlmqPagedKV *kv, const LlmqPa
   check_types(c, a->dtype, kv->dtype);
   c.require(a->n_rows >= 0 && a->n_seqs >= 0 && a->max_pages >= 0 && a->window >= 0, "negative size");
   c.require(a->n_heads > 0 && a->n_heads % kv->n_kv == 0, "n_heads must be a multiple of n_kv");
-  c.require((long long)a->max_pages * kv->page_size <= INT_MAX, "max_pages * page_size must stay below 2^31");
+  // (a tile may reach past the last position: room for it below 2^31)
+  c.require((long long)a->max_pages * kv->page_size <= INT_MAX - 4096, "max_pages * page_size must stay below 2^31 - 4096");
   c.require(a->table_stride >= a->max_pages, "table_stride is below max_pages");
   c.require(std::isfinite(a->scale), "scale is not finite");
   if (c.rc != LLMQ_OK || a->n_rows == 0) return c.rc;

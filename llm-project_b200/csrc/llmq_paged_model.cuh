@@ -39,12 +39,12 @@ void release_paged(LlmqPagedCache *c) {
   delete c;
 }
 
-// The cache behind a handle, with its model's GPU current; null if it is none.
-LlmqPagedCache *find_paged(const LlmqPagedCache *handle, const char *fn) {
+// The cache behind a handle, with its model's GPU current if `select`; null if it is none.
+LlmqPagedCache *find_paged(const LlmqPagedCache *handle, const char *fn, bool select) {
   for (auto &m : g_models)
     for (LlmqPagedCache *c : m.second->paged)
       if (c == handle) {
-        if (cudaSetDevice(c->model->device) == cudaSuccess) return c;
+        if (!select || cudaSetDevice(c->model->device) == cudaSuccess) return c;
         llmq_set_error(LLMQ_ERR_CUDA, "%s: cannot select device %d", fn, c->model->device);
         return nullptr;
       }
@@ -383,7 +383,7 @@ extern "C" LLMQ_API void q_llama_paged_free(LlmqPagedCache *handle) {
   if (!handle) return;
   int cur = -1;
   cudaGetDevice(&cur);
-  LlmqPagedCache *c = find_paged(handle, "q_llama_paged_free");
+  LlmqPagedCache *c = find_paged(handle, "q_llama_paged_free", true);
   if (c) {
     auto &v = c->model->paged;
     v.erase(std::remove(v.begin(), v.end(), c), v.end());
@@ -395,7 +395,7 @@ extern "C" LLMQ_API void q_llama_paged_free(LlmqPagedCache *handle) {
 
 extern "C" LLMQ_API int q_llama_paged_len(const LlmqPagedCache *handle, int seq) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
-  const LlmqPagedCache *c = find_paged(handle, "q_llama_paged_len");
+  const LlmqPagedCache *c = find_paged(handle, "q_llama_paged_len", false);
   if (!c) return -1;
   if (seq < 0 || seq >= c->max_seqs) {
     llmq_set_error(LLMQ_ERR_ARG, "q_llama_paged_len: sequence %d outside [0, %d)", seq, c->max_seqs);
@@ -406,13 +406,13 @@ extern "C" LLMQ_API int q_llama_paged_len(const LlmqPagedCache *handle, int seq)
 
 extern "C" LLMQ_API int q_llama_paged_free_pages(const LlmqPagedCache *handle) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
-  const LlmqPagedCache *c = find_paged(handle, "q_llama_paged_free_pages");
+  const LlmqPagedCache *c = find_paged(handle, "q_llama_paged_free_pages", false);
   return c ? static_cast<int>(c->free_list.size()) - c->head_h : -1;
 }
 
 extern "C" LLMQ_API int q_llama_paged_reset(LlmqPagedCache *handle, int seq) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
-  LlmqPagedCache *c = find_paged(handle, "q_llama_paged_reset");
+  LlmqPagedCache *c = find_paged(handle, "q_llama_paged_reset", true);
   if (!c) return q_llama_last_error();
   if (seq < 0 || seq >= c->max_seqs) {
     llmq_set_error(LLMQ_ERR_ARG, "q_llama_paged_reset: sequence %d outside [0, %d)", seq, c->max_seqs);
@@ -428,7 +428,7 @@ extern "C" LLMQ_API int q_llama_paged_reset(LlmqPagedCache *handle, int seq) {
 extern "C" LLMQ_API int q_llama_paged_step(const QLlamaModel *m, LlmqPagedCache *handle, const int *added,
                                            const int *tokens, const LlmqSampling *s, int *ids, Tensor *logits) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
-  LlmqPagedCache *c = find_paged(handle, "q_llama_paged_step");
+  LlmqPagedCache *c = find_paged(handle, "q_llama_paged_step", true);
   if (!c) return q_llama_last_error();
   return guarded("q_llama_paged_step", [&] { return paged_step(m, c, added, tokens, s, ids, logits); }, 0)
              ? LLMQ_OK

@@ -198,6 +198,8 @@ constexpr int kListBytes = kListCap * 8;
 constexpr int kWorkBytes = kListBytes + kHistBytes + kListBytes;
 static_assert(kHistBytes <= kListBytes, "regions are shared");
 
+constexpr int kMaxResident = 64 * 1024;  // of the slice
+
 struct RowArgs {
   LlmqSampleRows a;
   int slice;     // tokens a CTA, a multiple of 16
@@ -1448,9 +1450,12 @@ inline int scale_bits(int vocab) {
   return 62 - log2v < 50 ? 62 - log2v : 50;
 }
 
-// A launch of n_rows clusters of `ctas` CTAs, with programmatic dependent launch.
-cudaError_t launch_clusters(void (*kern)(RowArgs), const RowArgs &p, int ctas, int threads, int smem, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+// A launch of n_rows clusters of `ctas` CTAs, with programmatic dependent launch.  The
+// kernel's limit is set to the most any call takes, so that calls from several threads
+// do not lower it for one another.
+cudaError_t launch_clusters(void (*kern)(RowArgs), const RowArgs &p, int ctas, int threads, int smem, int most,
+                            cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(p.a.n_rows) * ctas);
@@ -1477,7 +1482,7 @@ cudaError_t launch_values(const LlmqSampleRows &a, int sms, cudaStream_t st) {
   p.slice = ((a.vocab + ctas - 1) / ctas + 15) / 16 * 16;
   const int own = (kPlaces + ctas - 1) / ctas;
   const int smem = (kPlaces + 3) / 4 * 16 + own * 12;
-  return launch_clusters(k_sample_values, p, ctas, kValueThreads, smem, st);
+  return launch_clusters(k_sample_values, p, ctas, kValueThreads, smem, (kPlaces + 3) / 4 * 16 + kPlaces * 12, st);
 }
 
 template <typename T>
@@ -1491,9 +1496,9 @@ cudaError_t launch(const LlmqSampleRows &a, int sms, cudaStream_t st) {
   auto slice_of = [&](int c) { return ((a.vocab + c - 1) / c + 15) / 16 * 16; };
   while (ctas < kMaxCluster && 2LL * a.n_rows * ctas <= 2 * sms && slice_of(ctas) > 2 * kThreads) ctas *= 2;
   p.slice = slice_of(ctas);
-  p.resident = p.slice * sizeof(T) <= 64 * 1024;  // beyond, two CTAs' slices do not fit an SM: from L2 each time
+  p.resident = p.slice * sizeof(T) <= kMaxResident;  // beyond, two CTAs' slices do not fit an SM: from L2 each time
   const int smem = kWorkBytes + (p.resident ? p.slice * (int)sizeof(T) : 0);
-  return launch_clusters(k_sample_rows<T>, p, ctas, kThreads, smem, st);
+  return launch_clusters(k_sample_rows<T>, p, ctas, kThreads, smem, kWorkBytes + kMaxResident, st);
 }
 
 }  // namespace

@@ -522,6 +522,58 @@ def test_attention_same_bits_again_and_on_other_streams(lib):
 
 
 @gpu
+@pytest.mark.parametrize("page", [2, 3, 8, 11, 40, 100, 129, 1000, 4097])
+@pytest.mark.parametrize("dtype,kv_dtype", [("f32", "f32"), ("f16", "f16")])
+def test_attention_page_sizes(lib, page, dtype, kv_dtype):
+    run_attend(lib, attend_state([1, 130, 1003], 4, 2, 64, page, dtype, kv_dtype), dtype, kv_dtype)
+
+
+@gpu
+def test_attention_more_rows_than_a_launch_takes(lib):
+    """1500 rows go in two launches that share the workspace."""
+    import torch
+    k, v, q, table, lens = attend_state([70, 33, 0, 129], 4, 2, 64, 16, "f32", "f32")
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn((1500, 4, 64), generator=g).cuda()
+    seqs = (torch.arange(1500) % 4).to(torch.int32).cuda()
+    lens = (torch.arange(1500) % 70).to(torch.int32).cuda().clamp(max=lens[seqs.long()])
+    run_attend(lib, (k, v, q, table, lens), "f32", "f32", seqs=seqs)
+
+
+@gpu
+def test_calls_of_two_threads_at_once(lib):
+    """Each thread on its own stream with its own buffers: the results of calls one by one."""
+    import threading
+
+    import torch
+    states = [attend_state([300, 7, 1200], 8, 2, 128, 16, *t) + (t,) for t in (("bf16", "bf16"), ("f32", "f32"))]
+    want = [attend_gpu(lib, k, v, t[1], q, table, lens, t[0]) for k, v, q, table, lens, t in states]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        k, v, q, table, lens, t = states[i]
+        st = torch.cuda.Stream()
+        out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        kv = describe_pool(k, v, t[1])
+        a, w = attend_descriptor(lib, k, q, out, table, lens, t[0], lse=lse)
+        torch.cuda.synchronize()
+        for _ in range(50):
+            if lib.llmq_paged_attention(C.byref(kv), C.byref(a), st.cuda_stream) != 0:
+                bad.append("error")
+        st.synchronize()
+        if not (torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])):
+            bad.append(i)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
+
+
+@gpu
 def test_host_memory_is_refused(lib):
     import torch
     k, v, q, table, lens = attend_state([9, 77], 4, 2, 64, 16, "f32", "f32")

@@ -211,6 +211,60 @@ def test_a_row_does_not_depend_on_its_batch(lib):
 
 
 @gpu
+def test_calls_of_several_threads_at_once(lib):
+    """Rows of different sizes and types, so that the calls' shared memory differs."""
+    import threading
+
+    import torch
+    g = np.random.default_rng(21)
+    jobs = [(V, t, torch.tensor(g.normal(0, 2, (3, V)), dtype=torch_type(t), device="cuda"))
+            for V, t in ((500, "f32"), (128256, "f32"), (40000, "f32"), (9000, "bf16"), (128256, "bf16"))]
+    s, u = (1.0, 0, 0.9, 0.0), [0.2, 0.5, 0.8]
+    want = [sample_gpu(lib, x, t, *s, u=u)[0].tolist() for _, t, x in jobs]
+    bad = []
+
+    def work(i):
+        f = dict(dtype=torch.float32, device="cuda")
+        _, t, x = jobs[i]
+        c = [torch.full((3,), v, **f) for v in (s[0], s[2])] + [torch.tensor(u, **f)]
+        ids = torch.zeros(3, dtype=torch.int32, device="cuda")
+        a = llmq.SampleRows(n_rows=3, vocab=x.shape[1], dtype=CODES[t], logits=ptr(x), stride=x.stride(0),
+                            temperature=ptr(c[0]), top_p=ptr(c[1]), u=ptr(c[2]), ids=ptr(ids))
+        st = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        for _ in range(50):
+            if lib.llmq_sample_rows(C.byref(a), st.cuda_stream) != 0:
+                bad.append("error")
+        st.synchronize()
+        if ids.tolist() != want[i]:
+            bad.append(i)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [300000, 1 << 20])
+def test_largest_vocabularies(lib, V, dtype):
+    import torch
+    g = np.random.default_rng(V)
+    x = torch.tensor(g.normal(0, 2, (1, V)), dtype=torch.float32).to(torch_type(dtype))
+    x[0, V - 1] = 11.0
+    row = x[0].double().numpy()
+    for s in [(1.0, 0, 1.0, 0.0), (0.8, 40, 0.95, 0.0), (1.0, 0, 0.7, 0.0), (1.0, 5000, 1.0, 0.0), (0.0, 0, 1.0, 0.0)]:
+        for u in (0.0, 0.4, 0.97):
+            i, _ = sample_gpu(lib, x.cuda(), dtype, *s, u=u)
+            want, _, margin = sample_plain(row, *[float(np.float32(v)) if n != 1 else v for n, v in enumerate(s)],
+                                           float(np.float32(u)))
+            assert margin < V * 2.0 ** -41 or i[0] == want, (s, u)
+
+
+@gpu
 def test_agrees_with_sample_token(lib):
     """The rows and settings of sample_token's own tests, with the u its stream gives:
     the same token wherever f32 sums cannot move the choice."""
