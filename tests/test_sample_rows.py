@@ -111,7 +111,8 @@ def test_large_vocabularies(lib, V, dtype):
 
 
 @gpu
-def test_awkward_rows(lib):
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_awkward_rows(lib, dtype):
     """Ties of whole rows, few distinct values, one word far above, a heavy tail, signed
     zeros, infinities, NaN, the type's lowest value, and nothing at all."""
     g = np.random.default_rng(9)
@@ -132,7 +133,28 @@ def test_awkward_rows(lib):
     rows = [np.full(V, 3.0), two, spike, zeros, masked, lowest, pinf, nan, np.full(V, -np.inf), np.full(V, np.nan),
             np.full(V, -big), ramp, ramp[::-1], np.where(np.arange(V) < 5000, 0.0, g.normal(-1, 0.1, V)),
             np.full(V, big), g.standard_cauchy(V)]
-    check_rows(lib, rows, "f32", SETTINGS, U)
+    check_rows(lib, rows, dtype, SETTINGS, U)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_rows_of_tiny_logits(lib, dtype):
+    """Logits of magnitudes far below the row's largest, on both sides of zero and with
+    zeros among them: a histogram of values holds them together."""
+    g = np.random.default_rng(10)
+    V = 5000
+    tiny = g.normal(0, 1e-6, V)
+    one = tiny.copy()
+    one[[17, 4000]] = 1.0
+    neg = tiny.copy()
+    neg[g.random(V) < 0.3] = -3.0
+    zeros = np.where(g.random(V) < 0.5, tiny, 0.0)
+    zeros[5] = 2.0
+    few = np.full(V, -5.0)
+    few[100:140] = np.linspace(-1e-5, 1e-5, 40)
+    few[7] = 0.5
+    spread = np.sign(g.normal(0, 1, V)) * 2.0 ** g.uniform(-40, 3, V)
+    check_rows(lib, [tiny, one, neg, zeros, few, spread], dtype, SETTINGS, U + [0.2, 0.35, 0.65])
 
 
 @gpu
