@@ -14,9 +14,8 @@ using namespace llmq;
 namespace {
 
 // ==================================================================== plan
-constexpr int kScanThreads = 1024;
-
-// Inclusive sum over the block's threads; *total receives the block's sum.
+// Inclusive sum over the block's NT threads; *total receives the block's sum.
+template <int NT>
 __device__ __forceinline__ long long block_scan(long long v, long long *warp_sums, long long *total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -27,13 +26,13 @@ __device__ __forceinline__ long long block_scan(long long v, long long *warp_sum
   __syncthreads();
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
-  long long w = warp_sums[lane];
+  long long w = lane < NT / 32 ? warp_sums[lane] : 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
+  for (int o = 1; o < NT / 32; o <<= 1) {
     const long long u = __shfl_up_sync(0xffffffffu, w, o);
     if (lane >= o) w += u;
   }
-  *total = __shfl_sync(0xffffffffu, w, 31);
+  *total = __shfl_sync(0xffffffffu, w, NT / 32 - 1);
   const long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
   return v + (warp ? before : 0);
 }
@@ -56,22 +55,24 @@ __device__ __forceinline__ void plan_row(const LlmqPagedPlan &a, int r, int seq,
   if (a.spans) a.spans[r] = pos + 1;
 }
 
-// A step of at most this many rows, over requests of one chunk, is done by the scanning
-// CTA alone: at 64 requests and rows the plan takes 4.4 us so and 7.5 us in two kernels,
-// at 4096 rows the two take the same.
-constexpr int kOneCtaRows = 4096;
+// What bounds a plan is latency: launches, and the chain of sums.  So a small step is done
+// by one CTA alone, rows and all; a larger one's rows take a second kernel (1000
+// requests with 1900 rows: 7.9 us in one, 8.1 us in two; 4800 rows: 11.0 and 9.0 us).
+constexpr int kOneCtaRows = 2048;
+// Up to this many requests and rows a CTA of 128 threads does, whose sums take fewer steps.
+constexpr int kSmallSeqs = 128, kSmallRows = 512;
 
-// One CTA: requests in chunks of 1024, one a thread.  Three sums in order:
-// rows over the requests of valid lengths (which of them fit max_rows), pages
-// over those (which fit the free pages), rows over what is served.  The chunk's
-// new pages are then written by all threads, each finding its request by
-// bisection of the page sums, and so are the rows of a small step.
-template <bool rows_too>
-__global__ void __launch_bounds__(kScanThreads) k_plan_scan(const LlmqPagedPlan a) {
+// One CTA: requests in chunks of NT, one a thread.  Sums in order: rows over the requests
+// of valid lengths (which of them fit max_rows), pages over those (which fit the free
+// pages), and, if a chunk refuses any, rows and pages over what is served (else those are
+// the first two).  The chunk's new pages are then written by all threads, each finding its
+// request by bisection of the page sums, and so are the rows of a small step.
+template <int NT, bool rows_too>
+__global__ void __launch_bounds__(NT) k_plan_scan(const LlmqPagedPlan a) {
   __shared__ long long s_warp[32];
-  __shared__ long long s_end[kScanThreads];  // page sums up to and with each request
-  __shared__ int s_have[kScanThreads], s_new[kScanThreads];
-  __shared__ int s_row_end[rows_too ? kScanThreads : 1], s_len[rows_too ? kScanThreads : 1];
+  __shared__ long long s_end[NT];  // page sums up to and with each request
+  __shared__ int s_have[NT], s_new[NT];
+  __shared__ int s_row_end[rows_too ? NT : 1], s_len[rows_too ? NT : 1];
   serve_wait();
   serve_dependents();
   const int tid = threadIdx.x;
@@ -79,31 +80,39 @@ __global__ void __launch_bounds__(kScanThreads) k_plan_scan(const LlmqPagedPlan 
   const bool bad_head = given_head < 0;
   const long long head = max(given_head, 0);
   const long long cap = (long long)a.max_pages * a.page_size;
+  const int page_size = a.page_size;
+  auto pages_of = [&](long long n) {  // n <= cap < 2^31
+    return static_cast<int>((static_cast<uint32_t>(n) + static_cast<uint32_t>(page_size) - 1u) / static_cast<uint32_t>(page_size));
+  };
   long long rows_seen = 0, pages_seen = 0, rows_done = 0, pages_done = 0;
   int flags = bad_head ? LLMQ_PAGED_NO_PAGES : 0;
-  for (int b0 = 0; b0 < a.n_seqs; b0 += kScanThreads) {
+  for (int b0 = 0; b0 < a.n_seqs; b0 += NT) {
     const int b = b0 + tid;
     const bool in = b < a.n_seqs;
     const long long cached = in ? a.cached[b] : 0, added = in ? a.added[b] : 0;
     const bool held = cached >= 0 && cached <= cap;
     const bool valid = held && added >= 0 && cached + added <= cap;
     if (in && !valid) flags |= LLMQ_PAGED_BAD_LEN;
-    long long total;
+    const int have = held ? pages_of(cached) : 0;
+    long long chunk_rows, chunk_pages;
     const long long want = valid ? added : 0;
-    const long long rows = rows_seen + block_scan(want, s_warp, &total);
-    rows_seen += total;
-    const bool fits = valid && (want == 0 || rows <= a.max_rows);
+    const long long rows = block_scan<NT>(want, s_warp, &chunk_rows);
+    const bool fits = valid && (want == 0 || rows_seen + rows <= a.max_rows);
     if (valid && !fits) flags |= LLMQ_PAGED_NO_ROWS;
-    const int page_size = a.page_size;
-    const int have = held ? static_cast<int>((cached + page_size - 1) / page_size) : 0;
-    const int need = fits ? static_cast<int>((cached + added + page_size - 1) / page_size) - have : 0;
-    const long long pages = pages_seen + block_scan(need, s_warp, &total);
-    pages_seen += total;
-    const bool served = fits && (need == 0 || (!bad_head && head + pages <= a.n_free));
+    const int need = fits ? pages_of(cached + added) - have : 0;
+    const long long pages = block_scan<NT>(need, s_warp, &chunk_pages);
+    const bool served = fits && (need == 0 || (!bad_head && head + pages_seen + pages <= a.n_free));
     if (fits && !served) flags |= LLMQ_PAGED_NO_PAGES;
+    rows_seen += chunk_rows;
+    pages_seen += chunk_pages;
     const long long mine = served ? added : 0;
-    const long long end = rows_done + block_scan(mine, s_warp, &total);
-    rows_done += total;
+    const int fresh = served ? need : 0;
+    long long row_sum = rows, page_sum = pages;
+    if (__syncthreads_or(in && !served && want > 0)) {
+      row_sum = block_scan<NT>(mine, s_warp, &chunk_rows);
+      page_sum = block_scan<NT>(fresh, s_warp, &chunk_pages);
+    }
+    const long long end = rows_done + row_sum;
     const int len = held ? static_cast<int>(cached + mine) : 0;
     if (in) {
       a.first[b] = static_cast<int>(end - mine);
@@ -113,14 +122,12 @@ __global__ void __launch_bounds__(kScanThreads) k_plan_scan(const LlmqPagedPlan 
       s_row_end[tid] = static_cast<int>(end);
       s_len[tid] = len;
     }
-    const int fresh = served ? need : 0;
-    const long long taken = pages_done + block_scan(fresh, s_warp, &total);
-    s_end[tid] = taken;
+    s_end[tid] = page_sum;
     s_have[tid] = have;
     s_new[tid] = fresh;
     __syncthreads();
-    for (long long j = pages_done + tid; j < pages_done + total; j += kScanThreads) {
-      int lo = 0, hi = kScanThreads - 1;  // the first request whose sum passes j
+    for (long long j = tid; j < chunk_pages; j += NT) {
+      int lo = 0, hi = NT - 1;  // the first request whose sum passes j
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (s_end[mid] > j)
@@ -129,9 +136,10 @@ __global__ void __launch_bounds__(kScanThreads) k_plan_scan(const LlmqPagedPlan 
           lo = mid + 1;
       }
       const int at = s_have[lo] + static_cast<int>(j - (s_end[lo] - s_new[lo]));
-      a.table[(long long)(b0 + lo) * a.table_stride + at] = a.free_pages[head + j];
+      a.table[(long long)(b0 + lo) * a.table_stride + at] = a.free_pages[head + pages_done + j];
     }
-    pages_done += total;
+    rows_done += chunk_rows;
+    pages_done += chunk_pages;
     __syncthreads();
   }
   if (tid == 0) {
@@ -140,8 +148,8 @@ __global__ void __launch_bounds__(kScanThreads) k_plan_scan(const LlmqPagedPlan 
   }
   if (flags && a.status) atomicOr(a.status, flags);
   if (rows_too)
-    for (int r = tid; r < a.max_rows; r += kScanThreads) {
-      int lo = 0, hi = kScanThreads - 1;  // the first request whose rows end behind r
+    for (int r = tid; r < a.max_rows; r += NT) {
+      int lo = 0, hi = NT - 1;  // the first request whose rows end behind r
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (s_row_end[mid] > r)
@@ -311,8 +319,11 @@ extern "C" LLMQ_API int llmq_paged_plan(const LlmqPagedPlan *a, void *stream) {
   c.memory(a->status, "status");
   if (c.rc != LLMQ_OK) return c.rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool one = a->n_seqs <= kScanThreads && a->max_rows <= kOneCtaRows;
-  c.launched(serve_launch(one ? k_plan_scan<true> : k_plan_scan<false>, dim3(1), dim3(kScanThreads), 0, st, *a));
+  const bool one = a->n_seqs <= 1024 && a->max_rows <= kOneCtaRows;
+  if (a->n_seqs <= kSmallSeqs && a->max_rows <= kSmallRows)
+    c.launched(serve_launch(k_plan_scan<128, true>, dim3(1), dim3(128), 0, st, *a));
+  else
+    c.launched(serve_launch(one ? k_plan_scan<1024, true> : k_plan_scan<1024, false>, dim3(1), dim3(1024), 0, st, *a));
   if (c.rc == LLMQ_OK && !one && a->max_rows > 0)
     c.launched(serve_launch(k_plan_fill, dim3((a->max_rows - 1) / kFillThreads + 1), dim3(kFillThreads), 0, st, *a));
   return c.rc;
