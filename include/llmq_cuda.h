@@ -635,7 +635,7 @@ typedef struct {
   int n_rows, n_heads;
   int dtype;     /* of q and out */
   int window;
-  int max_pages; /* entries of a table row */
+  int max_pages; /* entries of a table row; max_pages * page_size < 2^31 - 4096 */
   int n_seqs;    /* table rows */
   float scale;
   int reserved;
@@ -706,8 +706,8 @@ int q_llama_decode_batch_sample(const QLlamaModel *m, LlamaKV **kvs, const int *
 
 /* A paged cache of up to max_seqs sequences of a model: n_pages pages of
  * page_size positions (of every layer), shared out as the sequences grow, in
- * place of one max_seq cache a sequence.  dtype is the pages' type; sequences
- * start empty.  head_dim must be a multiple of 8, at most 256.  Not under tensor
+ * place of one max_seq cache a sequence (n_pages * page_size < 2^31 - 4096).
+ * dtype is the pages' type; sequences start empty.  head_dim must be a multiple of 8, at most 256.  Not under tensor
  * parallelism.  NULL on error.  The cache belongs to the model: freeing the model
  * frees it (the handle is then invalid). */
 typedef struct LlmqPagedCache LlmqPagedCache;

@@ -115,8 +115,9 @@ __global__ void __launch_bounds__(256) k_take_rows(const float *x, const int *la
 
 LlmqPagedCache *paged_create(const QLlamaModel *m, int n_pages, int page_size, int max_seqs, int dtype) {
   const char *fn = "q_llama_paged_create";
-  if (n_pages <= 0 || page_size <= 0 || max_seqs <= 0 || (long long)n_pages * page_size > INT_MAX || dtype < LLMQ_F32 ||
-      dtype > LLMQ_BF16) {
+  // (llmq_paged_attention's limit on a table row, so that no step is refused half way)
+  if (n_pages <= 0 || page_size <= 0 || max_seqs <= 0 || (long long)n_pages * page_size > INT_MAX - 4096 ||
+      dtype < LLMQ_F32 || dtype > LLMQ_BF16) {
     llmq_set_error(LLMQ_ERR_ARG, "%s: bad sizes or type (%d pages of %d, %d sequences)", fn, n_pages, page_size,
                    max_seqs);
     return nullptr;
@@ -179,9 +180,13 @@ LlmqPagedCache *paged_create(const QLlamaModel *m, int n_pages, int page_size, i
 
 int paged_reset(LlmqPagedCache *c, int seq) {
   std::vector<int> &own = c->pages[(size_t)seq];
+  std::vector<int> next;
   if (!own.empty()) {
-    std::vector<int> next(c->free_list.begin() + c->head_h, c->free_list.end());
+    next.assign(c->free_list.begin() + c->head_h, c->free_list.end());
     next.insert(next.end(), own.begin(), own.end());
+  }
+  c->broken = true;  // a failure from here on leaves the GPU's lists behind the host's
+  if (!own.empty()) {
     CK(upload_sync(c->free_pages, next.data(), next.size() * sizeof(int)));
     CK(zero_sync(c->head, sizeof(int)));
     c->free_list.swap(next);
@@ -190,6 +195,7 @@ int paged_reset(LlmqPagedCache *c, int seq) {
   }
   CK(zero_sync(c->lens + seq, sizeof(int)));
   c->len[(size_t)seq] = 0;
+  c->broken = false;
   return 1;
 }
 

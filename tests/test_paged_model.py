@@ -43,6 +43,15 @@ def test_refusals_without_a_gpu(lib):
         refused(lib, llmq.LLMQ_ERR_ARG, lib.q_llama_decode_batch_sample, C.byref(m), *args)
 
 
+def test_pages_that_attention_would_refuse(lib):
+    m = llmq.QLlamaModel(head_dim=64)
+    for n_pages, page in [(1, (1 << 31) - 4096), (1, (1 << 31) - 1), ((1 << 31) - 4000, 1)]:
+        lib.q_llama_clear_error()
+        assert lib.q_llama_paged_create(C.byref(m), n_pages, page, 1, llmq.LLMQ_BF16) is None
+        assert b"bad sizes" in lib.q_llama_last_error_message()
+    lib.q_llama_clear_error()
+
+
 # ------------------------------------------------------------------- GPU
 def step(lib, m, cache, added, tokens, seqs, s=None, want=True):
     n = sum(a > 0 for a in added)
