@@ -55,9 +55,11 @@ __device__ __forceinline__ void plan_row(const LlmqPagedPlan &a, int r, int seq,
   if (a.spans) a.spans[r] = pos + 1;
 }
 
-// What bounds a plan is latency: launches, and the chain of sums.  So a small step is done
-// by one CTA alone, rows and all; a larger one's rows take a second kernel (1000
-// requests with 1900 rows: 7.9 us in one, 8.1 us in two; 4800 rows: 11.0 and 9.0 us).
+// What bounds a plan is latency: launches, the chain of sums and of each search (64 requests
+// of one token 3.4 us; 1000 requests, 200 of them with prompts, some 100000 rows 11.3 us,
+// of which their 2.5 MB would take 0.4).  So a small step is done by one CTA alone, rows
+// and all; a larger one's rows take a second kernel (1000 requests with 1900 rows: 7.9 us
+// in one, 8.1 us in two; 4800 rows: 11.0 and 9.0 us).
 constexpr int kOneCtaRows = 2048;
 // Up to this many requests and rows a CTA of 128 threads does, whose sums take fewer steps.
 constexpr int kSmallSeqs = 128, kSmallRows = 512;
@@ -193,10 +195,15 @@ struct AppendArgs {
 constexpr int kAppendThreads = 256;
 constexpr int kHeadLanes = 8;
 
+// What bounds it: the rows' bytes, read once and written once.  16384 bf16 rows of 32 query
+// heads and 8 KV heads of 128 (404 MB) take 70.7 us, 5.7 TB/s of the 6.46 a plain copy
+// moves; 64 rows 3.3 us and one 1.9 us, the latency of a launch and two dependent loads.
+//
 // A thread owns VN adjacent pairs (d, d + head_dim / 2) of every `lanes`th head of a row:
 // the pairs' angles are read once and serve its heads.  The next head's loads are on
 // their way before a head is stored (q_out may be q, so the compiler may not move a load
-// over a store itself), the first head's before the row's slot is known.
+// over a store itself), the first head's before the row's slot is known.  Holding 2 to 6
+// heads' loads at once took registers and so warps: 85 to 177 us for those rows.
 template <typename T, typename KT, int VN>
 __global__ void __launch_bounds__(kAppendThreads) k_append(const AppendArgs p, int chunks, int lanes) {
   serve_wait();

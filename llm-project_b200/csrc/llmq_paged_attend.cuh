@@ -11,7 +11,7 @@
 // ends.  So one long row is split over all SMs, and ragged rows leave none
 // idle.  A CTA that covers a row's head from end to end writes the output; the at
 // most two shares that are cut (one at its beginning, one at its end) are left
-// in the workspace and joined by k_attend_join, one block for each head cut.
+// in the workspace and joined by k_attend_join, one block for each query head of a cut.
 //
 // In a CTA each warp owns a slice of every tile (kSlice positions) with its own
 // ring of kStages slices in shared memory, filled by 16-byte asynchronous
@@ -19,6 +19,19 @@
 // partial results are joined.  Positions past the row, before its window or on
 // a page outside the pool are filled with zeros and masked, so what memory
 // holds there (NaN too) is never used.
+//
+// Measured, both kernels (a plain copy moves 6.46 TB/s on the same GPU), 32 query heads
+// (the long row: 64) on 8 KV heads of 128:
+//   64 f32 rows of about 2100 positions      186 us, 5.98 TB/s (203 us under minutes of load)
+//   61 bf16 rows of up to 8191 positions     189 us, 5.94 TB/s
+//   one f16 row of 131072 positions           97 us, 5.52 TB/s: 6.95 TB/s in the long run
+//     and some 17 us that do not depend on the length (launch, prefix sums, the first
+//     loads' latency, the join)
+//   one row of a few hundred positions         7 us, the same chain without the bytes
+// Counters at 16 rows of 2100: the cache read once (280 MB of DRAM reads for 278 MB), 42%
+// (f32) and 33% (bf16) of the issue slots, 4 CTAs of 4 warps an SM or fewer (180 and 207
+// registers): the ring, not the warps, keeps the memory busy.
+// (One warp a row and head, plain loads and no split took 1794, 5016 and 57126 us.)
 #pragma once
 
 #include <climits>
