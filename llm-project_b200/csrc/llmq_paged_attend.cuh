@@ -29,7 +29,7 @@
 //     loads' latency, the join)
 //   one row of a few hundred positions         7 us, the same chain without the bytes
 // Counters at 16 rows of 2100: the cache read once (280 MB of DRAM reads for 278 MB), 42%
-// (f32) and 33% (bf16) of the issue slots, 4 CTAs of 4 warps an SM or fewer (180 and 207
+// (f32) and 33% (bf16) of the issue slots, 2 CTAs of 4 warps an SM (180 and 207
 // registers): the ring, not the warps, keeps the memory busy.
 // (One warp a row and head, plain loads and no split took 1794, 5016 and 57126 us.)
 #pragma once
