@@ -975,15 +975,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
 // eight times the values: it goes with the f32 ones.
 //
 // Measured: 256 rows of 128256 with nucleus, min-p and plain settings (65.7 MB, 10.2 us at
-// a plain copy's rate) 65.8 us: the two readings and the maximum 15, forming the indices
-// 15, the shared atomics 26 (8 were no two of a warp to meet in a bank), the cuts and the
-// draw 11.  The rows are read from DRAM once (65.9 MB), then from L2.
+// a plain copy's rate) 62.9 us.  Leaving parts out of a slightly slower form: the two readings
+// and the maximum 15, forming the indices 15, the shared atomics 26 (8 were no two of a
+// warp to meet in a bank), the cuts and the draw 11.  The rows are read from DRAM once (65.9 MB), then from L2.
 constexpr int kVals = 2048;
 // places, in falling order of their logits
 constexpr int kTinyPos = kVals, kZeroAt = kVals + 1, kTinyNeg = kVals + 2, kNeg0 = kVals + 3;
 constexpr int kPlaces = 2 * kVals + 3;
 constexpr int kValueThreads = 512;
-constexpr int kAhead = 3;  // vectors of 16 bytes a thread has in flight while it counts as many
+// Vectors of 16 bytes a thread has in flight while it counts as many: 256 rows of 128256 take
+// 62.9 us with 2, 67.6 with 3 (registers spill).
+constexpr int kAhead = 2;
 
 // Where a place is counted: positive magnitudes upwards, then negative ones upwards
 // and the three about zero, so that a token's index is its bits and one product away.
@@ -1192,11 +1194,14 @@ __global__ void __launch_bounds__(kValueThreads, 2) k_sample_values(const RowArg
       int near = 0;
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) near |= add2(x[i].x) | add2(x[i].y) | add2(x[i].z) | add2(x[i].w);
-      if (near < 0) {  // seldom: read them again
+      if (near < 0) {  // seldom: look at them again (reading them again, one by one, took 3 us more)
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {  // (what is past the end is NaN: passed over)
+          const uint4 y = x[i];
 #pragma unroll 1
-        for (int i = 0; i < kAhead; ++i)
-#pragma unroll 1
-          for (int e = 0; e < 8 && v + i * kValueThreads < nv; ++e) add_near(row[head + 8 * (v + i * kValueThreads) + e]);
+          for (int e = 0; e < 8; ++e)
+            add_near(((e < 4 ? e < 2 ? y.x : y.y : e < 6 ? y.z : y.w) >> (16 * (e & 1))) & 0xffffu);
+        }
       }
     }
 #pragma unroll 1
@@ -1490,6 +1495,8 @@ cudaError_t launch_values(const LlmqSampleRows &a, int sms, cudaStream_t st) {
   RowArgs p{};
   p.a = a;
   p.scale = scale_bits(a.vocab);
+  // CTAs a row until every SM has one: 128 rows 39 us in clusters of 2, 48 of 4; 256 rows
+  // 66 us alone, 73 in clusters of 2
   int ctas = 1;
   while (ctas < kMaxCluster && (long long)a.n_rows * ctas < sms && a.vocab / ctas > 4 * kValueThreads) ctas *= 2;
   p.slice = ((a.vocab + ctas - 1) / ctas + 15) / 16 * 16;

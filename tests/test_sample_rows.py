@@ -138,6 +138,30 @@ def test_awkward_rows(lib, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_min_p_without_top_p(lib, dtype):
+    """What min_p asks for can be bounded beforehand: rows whose bound lies above zero, at
+    it and below it, with NaN, infinities and the type's lowest value among them."""
+    g = np.random.default_rng(12)
+    V, big = 9001, np.finfo(np.float32).max
+    x = g.normal(0, 2, V)
+    holes = x + 6
+    holes[::5], holes[1::5], holes[2::5] = np.nan, -np.inf, -big
+    zero = np.where(g.random(V) < 0.5, x, 0.0)
+    zero[zero > 0] = 0.0
+    zero[[3, 8000]] = np.log(20.0)  # with min_p 0.05 the bound is next to 0
+    tiny = g.normal(0, 1e-7, V)
+    tiny[11] = 1e-6
+    pinf = x.copy()
+    pinf[[70, 4]] = np.inf
+    rows = [x + 10, x - 10, x, holes, zero, tiny, tiny - 1, pinf, np.full(V, 7.0), np.full(V, -7.0), 40 * x]
+    settings = [(1.0, 0, 1.0, 0.05), (1.0, 20, 1.0, 0.05), (1.0, 3000, 0.0, 0.001), (0.5, 0, 1.0, 1e-30),
+                (3.0, 50, 0.0, 0.3), (float("inf"), 0, 1.0, 1.0), (float("inf"), 7, 1.0, 0.5), (1.0, 0, 1.0, 1.0),
+                (0.01, 2, 1.0, 0.5), (20.0, 0, 1.0, 0.9)]
+    check_rows(lib, rows, dtype, settings, U)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_rows_of_tiny_logits(lib, dtype):
     """Logits of magnitudes far below the row's largest, on both sides of zero and with
     zeros among them: a histogram of values holds them together."""
