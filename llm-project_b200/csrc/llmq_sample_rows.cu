@@ -29,7 +29,7 @@
 // What bounds it is not DRAM but instructions and latency: a weight costs some 30
 // instructions (doubles, for the exact sum), the histogram two shared atomics a token.
 // Measured: 64 f32 rows of 128256 with mixed settings (32.8 MB, 5.1 us at a plain copy's
-// rate) 52.6 us, the rows without a bound last longest; the same rows with a top_k of 50,
+// rate) 52.4 us, the rows without a bound last longest; the same rows with a top_k of 50,
 // no exponential but the list's, 24 us; one row of 32000, top_k 40 and top_p, 10.6 us, a
 // chain of cluster barriers.  Counters for the mixed rows: 33.0 MB read, 40% of the issue
 // slots, two further turns of a shared atomic for equal banks.
