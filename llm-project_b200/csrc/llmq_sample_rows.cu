@@ -81,33 +81,44 @@ struct RowRule {
 
   uint32_t far;        // high word of 256 (S + 1): a y from there on has a w that rounds to 0
 
-  // w * 2^S before rounding; *counts: it does not round to 0 (false for NaN and
-  // -infinity; the value is then nothing).  Not for an infinite maximum.
-  __device__ __forceinline__ double share_near(float l, bool *counts) const {
-    const double y = (mxd - static_cast<double>(l)) * step;  // >= 0, or NaN
-    const double yr = y + 6755399441055744.0;  // 1.5 * 2^52: the integer in the low bits
-    const int n = __double2loint(yr);
-    const double x = y - (yr - 6755399441055744.0);
-    constexpr double c = -2.7076061740622863e-3;  // -ln 2 / 256
-    double p = fma(x, c * c * c * c / 24.0, c * c * c / 6.0);
-    p = fma(x, p, c * c / 2.0);
-    p = fma(x, p, c);
-    p = fma(x, p, 1.0);
-    const double t = tab[n & (kExpTable - 1)];  // of 2^S 2^(-i / 256)
-    *counts = static_cast<uint32_t>(__double2hiint(y)) < far;  // as unsigned: no NaN of either sign
-    return p * __hiloint2double(__double2hiint(t) - ((n >> 8) << 20), __double2loint(t));
-  }
-  __device__ __forceinline__ double share(float l) const {
-    if (infinite) return l == mx ? __hiloint2double((1023 + scale) << 20, 0) : 0.0;
+  // w * 2^S before rounding, as a product; counts: it does not round to 0 (false for NaN
+  // and -infinity; the product is then nothing).
+  //
+  // A token's weight is formed at several places (histogram, whole sum, list, divided step),
+  // whose sums have to agree to the unit.  So each operation names its rounding: left to
+  // the compiler, which may make one operation of a product and a sum at one place and
+  // two at another, one weight in 70 could differ by a unit.
+  struct Product {
+    double p, t;
     bool counts;
-    const double s = share_near(l, &counts);
-    return counts ? s : 0.0;
+  };
+  static constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: the integer in the low bits
+  __device__ __forceinline__ Product product(float l) const {  // not for an infinite maximum
+    const double y = __dmul_rn(__dsub_rn(mxd, static_cast<double>(l)), step);  // >= 0, or NaN
+    const double yr = __dadd_rn(y, kRound);
+    const int n = __double2loint(yr);
+    const double x = __dsub_rn(y, __dsub_rn(yr, kRound));
+    constexpr double c = -2.7076061740622863e-3;  // -ln 2 / 256
+    double p = __fma_rn(x, c * c * c * c / 24.0, c * c * c / 6.0);
+    p = __fma_rn(x, p, c * c / 2.0);
+    p = __fma_rn(x, p, c);
+    p = __fma_rn(x, p, 1.0);
+    const double t = tab[n & (kExpTable - 1)];  // of 2^S 2^(-i / 256)
+    const bool counts = static_cast<uint32_t>(__double2hiint(y)) < far;  // as unsigned: no NaN of either sign
+    return Product{p, __hiloint2double(__double2hiint(t) - ((n >> 8) << 20), __double2loint(t)), counts};
   }
-  static __device__ __forceinline__ u64 round(double s) {
-    const double r = s + 6755399441055744.0;  // s < 2^51
-    return static_cast<u64>(__double_as_longlong(r)) - 0x4338000000000000ull;
+  // the product next to an integer, rounded once (it is below 2^51)
+  static __device__ __forceinline__ u64 rounded(const Product &e) {
+    return static_cast<u64>(__double_as_longlong(__fma_rn(e.p, e.t, kRound))) - 0x4338000000000000ull;
   }
-  __device__ __forceinline__ u64 weight(float l) const { return round(share(l)); }
+  __device__ __forceinline__ Product product_any(float l) const {
+    if (infinite) return Product{1.0, __hiloint2double((1023 + scale) << 20, 0), l == mx};
+    return product(l);
+  }
+  __device__ __forceinline__ double share(const Product &e) const { return e.counts ? __dmul_rn(e.p, e.t) : 0.0; }
+  __device__ __forceinline__ u64 weight(const Product &e) const { return e.counts ? rounded(e) : 0ull; }
+  __device__ __forceinline__ double share(float l) const { return share(product_any(l)); }
+  __device__ __forceinline__ u64 weight(float l) const { return weight(product_any(l)); }
   // the histogram's step: any function that does not fall as l falls will do (the
   // integer next to the product; NaN goes last)
   __device__ __forceinline__ int bin(float l) const {
@@ -153,7 +164,11 @@ struct Shared {
   uint32_t pick_key;
   int pick_bin, pick_count;
   u64 pick_before, pick_before_count;
-  int pick_item;
+  int pick_item;     // of a greedy row
+  int found[2];      // a list's item, -1: none (the calls take the places in turn)
+  u64 found_sum[2];
+  int last;          // the list's last item of a weight, and its sum
+  u64 last_sum;
   u64 sum, tokens;
   Step step[4];  // the top_p cut's, the top_k's, the least and the most the draw can be in
   Command cmd;
@@ -167,9 +182,10 @@ __device__ __forceinline__ u64 warp_scan(u64 v) {
   }
   return v;
 }
-// Inclusive sum over the block's threads; every thread of the block calls this.
+// Inclusive sum over the block's threads (*all: of all of them); every thread of the
+// block calls this.
 template <int NT = kThreads>
-__device__ __forceinline__ u64 block_scan(u64 v, u64 *red) {
+__device__ __forceinline__ u64 block_scan(u64 v, u64 *red, u64 *all = nullptr) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v = warp_scan(v);
   __syncthreads();
@@ -177,6 +193,7 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64 *red) {
   __syncthreads();
   const u64 w = warp_scan(lane < NT / 32 ? red[lane] : 0);
   const u64 before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  if (all) *all = __shfl_sync(0xffffffffu, w, 31);
   return warp ? v + before : v;
 }
 __device__ __forceinline__ u64 block_sum(u64 v, u64 *red) {
@@ -238,6 +255,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   if (tid == 0) {
     sh.listed = sh.total = 0;
     sh.pick_item = INT_MAX;
+    sh.found[0] = sh.found[1] = -1;
+    sh.last = 0;
+    sh.last_sum = 0;
   }
   serve_wait();
   serve_dependents();
@@ -477,12 +497,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (all.value) {
-            const double s = rule.share(l[h + i]);
-            w[i] = RowRule::round(s);
+            const RowRule::Product e = rule.product_any(l[h + i]);
+            w[i] = rule.weight(e);
             counts[i] = w[i] != 0;
-            above += s >= min_share ? w[i] : 0;
+            above += rule.share(e) >= min_share ? w[i] : 0;
           } else {
-            w[i] = RowRule::round(rule.share_near(l[h + i], &counts[i]));
+            const RowRule::Product e = rule.product(l[h + i]);
+            w[i] = RowRule::rounded(e);
+            counts[i] = e.counts;
           }
           b[i] = rule.bin(l[h + i]);
         }
@@ -605,25 +627,36 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       w[i] = x < m ? rule.weight(key_logit(static_cast<uint32_t>(items[x] >> kIndexBits))) : 0;
       mine += w[i];
     }
-    u64 at = before + block_scan(mine, sh.red) - mine;
+    u64 all;  // of the list
+    u64 at = before + block_scan(mine, sh.red, &all) - mine;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       at += w[i];
       sums[i] = at;
+      if (w[i] && at == before + all) {
+        sh.last = tid * kPer + i;
+        sh.last_sum = at;
+      }
     }
   };
-  // one thread's item, known to it, and its sum to all
+  // One thread's item, known to it, and its sum to all; if no thread has it (which sums
+  // that agree rule out), the last item of a weight: always one of the list.
+  int calls = 0;
   auto share_item = [&](auto is_it, u64 *sum_there) -> int {
+    const int mine = calls & 1;
+    ++calls;
     __syncthreads();
+    if (tid == 0) sh.found[mine ^ 1] = -1;  // for the next call: the last one's is read
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (is_it(i)) {
-        sh.pick_item = tid * kPer + i;
-        sh.pick_before = sums[i];
+        sh.found[mine] = tid * kPer + i;
+        sh.found_sum[mine] = sums[i];
       }
     __syncthreads();
-    *sum_there = sh.pick_before;
-    return sh.pick_item;
+    const int item = sh.found[mine];
+    *sum_there = item < 0 ? sh.last_sum : sh.found_sum[mine];
+    return item < 0 ? sh.last : item;
   };
   // the first of the list's items whose sum reaches target (there is one), and its sum
   auto reach = [&](u64 target, u64 *sum_there) {
@@ -841,7 +874,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
     return;
   }
   // The step of `mass` / `count` in which the measure reaches target, from `before`
-  // (sums) and `before_n` (tokens) on.
+  // (sums) and `before_n` (tokens) on; a target outside what the steps hold (which sums
+  // that agree rule out) is the first or the last of them.
   auto find_step = [&](const u64 *mass, const uint32_t *count, bool by_count, u64 target, u64 before, u64 before_n) {
     u64 m[kBins / kThreads], c[kBins / kThreads], ms = 0, cs = 0;
 #pragma unroll
@@ -851,8 +885,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
       ms += m[i];
       cs += c[i];
     }
-    u64 am = before + block_scan(ms, sh.red) - ms;
-    u64 ac = before_n + block_scan(cs, sh.red) - cs;
+    u64 all_m, all_c;
+    u64 am = before + block_scan(ms, sh.red, &all_m) - ms;
+    u64 ac = before_n + block_scan(cs, sh.red, &all_c) - cs;
+    const u64 from = by_count ? before_n : before, all = by_count ? all_c : all_m;
+    target = min(max(target, from + 1), from + max(all, 1ull));
 #pragma unroll
     for (int i = 0; i < kBins / kThreads; ++i) {
       const u64 has = by_count ? ac : am, gets = has + (by_count ? c[i] : m[i]);
@@ -870,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   // Lists the tokens around where the measure reaches target; returns the item there,
   // *sum_there the row's sum up to and with it.  If all tokens up to there fit the
   // list, they are listed and *from_start is set.
-  auto select = [&](bool by_count, u64 target, bool *from_start, u64 *sum_there) {
+  auto select = [&](bool by_count, u64 target, bool *from_start, u64 *sum_there) __attribute__((always_inline)) {
     find_step(tot_mass, tot_count, by_count, target, 0, 0);
     Command c{};
     c.bin0 = c.bin1 = sh.pick_bin;
@@ -1169,8 +1206,8 @@ __global__ void __launch_bounds__(kValueThreads, 2) k_sample_values(const RowArg
       ++zeros;
       return;
     }
-    const double s = rule.share(bf16_bits(b));
-    const u64 w = RowRule::round(s), v = s >= min_share ? w : 0;
+    const RowRule::Product e = rule.product_any(bf16_bits(b));
+    const u64 w = rule.weight(e), v = rule.share(e) >= min_share ? w : 0;
     if (b & 0x8000u) {
       ++neg_n;
       neg_m += w;
@@ -1244,9 +1281,9 @@ __global__ void __launch_bounds__(kValueThreads, 2) k_sample_values(const RowArg
       const uint32_t c = total[i];
       u64 m = 0, v = 0;
       if (c && one_value(p0 + i)) {
-        const double s = rule.share(value_at(p0 + i));
-        m = c * RowRule::round(s);
-        v = s >= min_share ? m : 0;
+        const RowRule::Product e = rule.product_any(value_at(p0 + i));
+        m = c * rule.weight(e);
+        v = rule.share(e) >= min_share ? m : 0;
       } else if (c) {
         for (int q = 0; q < ctas; ++q) {
           const ValueShared *o = cluster.map_shared_rank(&sh, q);
