@@ -753,7 +753,7 @@ struct DevModel {
   std::vector<cudaEvent_t> *prof = nullptr;
   // multi-row passes (batched decode, prefill): grow-only scratch
   struct Rows {
-    int cap = 0, lm_cap = 0;
+    int cap = 0, scores_cap = 0, lm_cap = 0;
     float *x = nullptr, *qkv = nullptr, *qr = nullptr, *ao = nullptr, *h = nullptr, *scores = nullptr;
     float *logits = nullptr, *logits_all = nullptr;  // logits_all: gathered shards (tensor parallel)
     float *tp_max = nullptr;                         // [rows] reduced absmax (tensor parallel)
@@ -1711,14 +1711,16 @@ int reset_after_device_error(DevModel *M, int flags) {
 // ------------------------------------------------------- multi-row passes
 constexpr int kRowsPerPass = 1024;  // rows of one pass (longer prompts run in several)
 
-int ensure_rows(DevModel *M, int rows, int lm_rows) {
+// `scores`: of the contiguous caches' attention (rows x n_heads x max_seq), which a pass
+// over pages or of the lm-head alone does without.
+int ensure_rows(DevModel *M, int rows, int lm_rows, bool scores) {
   auto &R = M->rows;
   const LlmqConfig &cfg = M->cfg;
   if (rows > R.cap) {
-    void *old[] = {R.x, R.qkv, R.qr, R.ao, R.h, R.scores, R.rd, R.tp_max};
+    void *old[] = {R.x, R.qkv, R.qr, R.ao, R.h, R.rd, R.tp_max};
     for (void *p : old) cudaFree(p);
     cudaFreeHost(R.h_rd);
-    R.x = R.qkv = R.qr = R.ao = R.h = R.scores = R.tp_max = nullptr;
+    R.x = R.qkv = R.qr = R.ao = R.h = R.tp_max = nullptr;
     R.rd = nullptr;
     R.h_rd = nullptr;
     R.cap = 0;
@@ -1728,11 +1730,17 @@ int ensure_rows(DevModel *M, int rows, int lm_rows) {
     CK(cudaMalloc(&R.qr, n * M->qd * sizeof(float)));
     CK(cudaMalloc(&R.ao, n * M->qd * sizeof(float)));
     CK(cudaMalloc(&R.h, n * cfg.d_ff * sizeof(float)));
-    CK(cudaMalloc(&R.scores, n * cfg.n_heads * cfg.max_seq * sizeof(float)));
     CK(cudaMalloc(&R.rd, n * sizeof(RowDesc)));
     CK(cudaMalloc(&R.tp_max, n * sizeof(float)));
     CK(cudaMallocHost(&R.h_rd, n * sizeof(RowDesc)));
     R.cap = rows;
+  }
+  if (scores && rows > R.scores_cap) {
+    cudaFree(R.scores);
+    R.scores = nullptr;
+    R.scores_cap = 0;
+    CK(cudaMalloc(&R.scores, (size_t)rows * cfg.n_heads * cfg.max_seq * sizeof(float)));
+    R.scores_cap = rows;
   }
   if (lm_rows > R.lm_cap) {
     cudaFree(R.logits);
@@ -1779,7 +1787,7 @@ int run_rows(DevCtx &c, DevModel *M, const RowDesc *rows_h, int rows, int lm0, f
 
   const int dm = cfg.d_model, qd = M->qd, kvd = M->kvd, hd = cfg.head_dim, dff = cfg.d_ff;
   const int lm_rows = rows - lm0;
-  if (!ensure_rows(M, rows, lm_rows)) return 0;
+  if (!ensure_rows(M, rows, lm_rows, !hook.paged && !hook.x)) return 0;
   auto &R = M->rows;
   int max_kpad = M->lm.Kpad;
   for (int l = 0; l < cfg.n_layers; ++l)

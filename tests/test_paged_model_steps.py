@@ -1,0 +1,31 @@
+"""Steps over a paged cache beside their results: the memory they take, what a refused one
+leaves, and what they wait for."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import llmq
+from helpers import TINY, synth
+from test_paged_model import refused, step
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+def test_a_step_takes_no_memory_for_contiguous_attention(lib):
+    """500 rows at max_seq 36000: the contiguous path's scores would take 430 MB, the rows
+    themselves 5 MB."""
+    import torch
+    m = synth(lib, dict(TINY, max_seq=36000, n_layers=1), seed=11)
+    cache = lib.q_llama_paged_create(C.byref(m), 40, 16, 2, llmq.LLMQ_BF16)
+    llmq.check(lib)
+    tokens = np.random.default_rng(5).integers(0, m.vocab, 500).tolist()
+    step(lib, m, cache, [1, 1], tokens[:2], 2)  # what any step needs once
+    before = torch.cuda.mem_get_info()[0]
+    step(lib, m, cache, [500, 0], tokens, 2)
+    assert before - torch.cuda.mem_get_info()[0] < 100 << 20
+    lib.q_llama_paged_free(cache)
+    lib.q_llama_model_free(C.byref(m))
