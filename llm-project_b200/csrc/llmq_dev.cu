@@ -32,12 +32,20 @@ extern "C" const uint32_t llmq_expf_exceptions_count;
   do {                                                                                                 \
     cudaError_t e_ = (call);                                                                           \
     if (e_ != cudaSuccess) {                                                                           \
-      llmq_set_error(LLMQ_ERR_CUDA, "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); \
+      set_cuda_error(e_, #call, __FILE__, __LINE__);                                                   \
       return 0;                                                                                        \
     }                                                                                                  \
   } while (0)
 
 namespace {
+
+// The error of a failed call.  An allocation that does not fit is LLMQ_ERR_OOM, and the
+// runtime forgets it: nothing later stumbles over it.
+void set_cuda_error(cudaError_t e, const char *call, const char *file, int line) {
+  if (e == cudaErrorMemoryAllocation) cudaGetLastError();
+  llmq_set_error(e == cudaErrorMemoryAllocation ? LLMQ_ERR_OOM : LLMQ_ERR_CUDA, "%s: %s (%s:%d)", call,
+                 cudaGetErrorString(e), file, line);
+}
 
 constexpr int kMaxDevices = 64;
 

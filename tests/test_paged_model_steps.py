@@ -29,3 +29,16 @@ def test_a_step_takes_no_memory_for_contiguous_attention(lib):
     assert before - torch.cuda.mem_get_info()[0] < 100 << 20
     lib.q_llama_paged_free(cache)
     lib.q_llama_model_free(C.byref(m))
+
+
+@gpu
+def test_a_pool_that_does_not_fit_is_out_of_memory(lib):
+    """One page of 2^31 - 8192 positions of 96 floats: some 800 GB, refused by the allocator
+    at once.  A smaller cache and its steps work afterwards."""
+    m = synth(lib, dict(TINY, n_layers=1), seed=12)
+    refused(lib, llmq.LLMQ_ERR_OOM, lambda: lib.q_llama_paged_create(C.byref(m), 1, (1 << 31) - 8192, 1, llmq.LLMQ_F32))
+    cache = lib.q_llama_paged_create(C.byref(m), 2, 16, 1, llmq.LLMQ_F32)
+    llmq.check(lib)
+    step(lib, m, cache, [3], [1, 2, 3], 1)
+    lib.q_llama_paged_free(cache)
+    lib.q_llama_model_free(C.byref(m))
