@@ -1773,6 +1773,17 @@ int ensure_rows(DevModel *M, int rows, int lm_rows, bool scores) {
   return 1;
 }
 
+// What a pass of `rows` rows, `lm_rows` of them for the lm-head, holds beside its products' sums.
+int ensure_pass(DevCtx &c, DevModel *M, int rows, int lm_rows, bool scores) {
+  if (!ensure_rows(M, rows, lm_rows, scores)) return 0;
+  int max_kpad = M->lm.Kpad;
+  for (int l = 0; l < M->cfg.n_layers; ++l)
+    max_kpad = std::max({max_kpad, M->qkv[l].Kpad, M->wo[l].Kpad, M->w13[l].Kpad, M->w2[l].Kpad});
+  const int n_rb = (rows + kTcRows - 1) / kTcRows;
+  return ensure(&c.tc_codes, &c.tc_codes_n, (size_t)n_rb * kTcRows * max_kpad, false) &&
+         ensure(&c.tc_as, &c.tc_as_n, (size_t)n_rb * kTcRows, false);
+}
+
 // What a pass does differently: over a paged cache its rows' keys, values and
 // attention go through the pages; rows of the residual stream given apart skip the
 // layers; the next tokens of the lm-head's rows are drawn instead of the greedy ids.
@@ -1795,15 +1806,8 @@ int run_rows(DevCtx &c, DevModel *M, const RowDesc *rows_h, int rows, int lm0, f
 
   const int dm = cfg.d_model, qd = M->qd, kvd = M->kvd, hd = cfg.head_dim, dff = cfg.d_ff;
   const int lm_rows = rows - lm0;
-  if (!ensure_rows(M, rows, lm_rows, !hook.paged && !hook.x)) return 0;
+  if (!ensure_pass(c, M, rows, lm_rows, !hook.paged && !hook.x)) return 0;
   auto &R = M->rows;
-  int max_kpad = M->lm.Kpad;
-  for (int l = 0; l < cfg.n_layers; ++l)
-    max_kpad = std::max({max_kpad, M->qkv[l].Kpad, M->wo[l].Kpad, M->w13[l].Kpad, M->w2[l].Kpad});
-  const int n_rb = (rows + kTcRows - 1) / kTcRows;
-  if (!ensure(&c.tc_codes, &c.tc_codes_n, (size_t)n_rb * kTcRows * max_kpad, false) ||
-      !ensure(&c.tc_as, &c.tc_as_n, (size_t)n_rb * kTcRows, false))
-    return 0;
   std::memcpy(R.h_rd, rows_h, (size_t)rows * sizeof(RowDesc));
   CK(cudaMemcpyAsync(R.rd, R.h_rd, (size_t)rows * sizeof(RowDesc), cudaMemcpyHostToDevice, st));
 

@@ -199,6 +199,23 @@ int paged_reset(LlmqPagedCache *c, int seq) {
   return 1;
 }
 
+// Everything a step of T rows, n_active of them for the lm-head, would allocate on its way.
+int paged_reserve(DevCtx &ctx, DevModel *M, int T, int n_active) {
+  const LlmqConfig &cfg = M->cfg;
+  TcArgs t;
+  // a full pass, if there is one, and the last
+  for (int rows : {std::min(T, kRowsPerPass), T % kRowsPerPass}) {
+    if (rows == 0) continue;
+    if (!ensure_pass(ctx, M, rows, 0, false)) return 0;
+    for (int l = 0; l < cfg.n_layers; ++l)
+      for (const Mat *w : {&M->qkv[l], &M->wo[l], &M->w13[l], &M->w2[l]})
+        if (!plan_tc(ctx, *w, rows, t)) return 0;
+  }
+  for (int rows : {std::min(n_active, kRowsPerPass), n_active % kRowsPerPass})
+    if (rows > 0 && (!ensure_pass(ctx, M, rows, rows, false) || !plan_tc(ctx, M->lm, rows, t))) return 0;
+  return 1;
+}
+
 int paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const int *tokens, const LlmqSampling *s,
                int *ids, Tensor *logits) {
   const char *fn = "q_llama_paged_step";
@@ -277,6 +294,12 @@ int paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const 
     CK(cudaMalloc(&c->spans, (size_t)T * sizeof(int)));
     c->cap = T;
   }
+  LlmqSampleRows limits{};
+  limits.vocab = cfg.vocab;
+  limits.dtype = LLMQ_F32;
+  if (s && llmq_sample_rows(&limits, M->stream) != LLMQ_OK) return 0;  // (no rows: its checks alone)
+  if (!paged_reserve(*ctx, M, T, n_active)) return 0;
+  std::vector<int> drawn((size_t)n_active);
   SampleColumns cols;
   if (s && !cols.fill(*s, n_active, active.data(), M->stream)) return 0;
   CK(upload_sync(c->added, added, (size_t)c->max_seqs * sizeof(int)));
@@ -314,7 +337,6 @@ int paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const 
     CK(launch_pdl(k_take_rows, dim3(n_active), dim3(256), 0, M->stream, static_cast<const float *>(M->rows.x),
                   static_cast<const int *>(c->last), off, n, cfg.d_model, c->x));
   }
-  std::vector<int> drawn((size_t)n_active);
   for (int off = 0; off < n_active; off += kRowsPerPass) {
     const int n = std::min(kRowsPerPass, n_active - off);
     RowsHook hook;
