@@ -771,6 +771,9 @@ struct DevModel {
     RowDesc *h_rd = nullptr;  // pinned
     int *h_ids = nullptr;     // pinned
     int *h_err = nullptr;     // pinned
+    // sampling settings, five columns of up to sample_cap sequences
+    size_t sample_cap = 0;
+    float *sample = nullptr, *h_sample = nullptr;  // h_sample: pinned
   } rows;
 };
 
@@ -818,8 +821,9 @@ void release_model(DevModel *M) {
   for (void *p : dev_ptrs) cudaFree(p);
   {
     auto &R = M->rows;
-    void *rp[] = {R.x, R.qkv, R.qr, R.ao, R.h, R.scores, R.logits, R.logits_all, R.tp_max, R.rd, R.ids, R.argmax};
+    void *rp[] = {R.x, R.qkv, R.qr, R.ao, R.h, R.scores, R.logits, R.logits_all, R.tp_max, R.rd, R.ids, R.argmax, R.sample};
     for (void *p : rp) cudaFree(p);
+    cudaFreeHost(R.h_sample);
     cudaFreeHost(R.h_rd);
     cudaFreeHost(R.h_ids);
     cudaFreeHost(R.h_err);
@@ -1980,27 +1984,35 @@ int run_rows(DevCtx &c, DevModel *M, const RowDesc *rows_h, int rows, int lm0, f
   return 1;
 }
 
-// Sampling settings of n sequences on the GPU, in columns.
+// Sampling settings of n sequences on the GPU, in columns: in buffers of the model that
+// only grow (cudaFree would wait for all that runs on the GPU, each step), copied on its
+// stream.  Steps of a model follow one another, so the last one's copy is done.
 struct SampleColumns {
-  float *dev = nullptr;
+  const float *dev = nullptr;
   size_t n = 0;
   bool has[5] = {};
-  SampleColumns() = default;
-  SampleColumns(const SampleColumns &) = delete;
-  ~SampleColumns() { cudaFree(dev); }
   // of the sequences listed in `which` (null: 0 .. count)
-  int fill(const LlmqSampling &s, int count, const int *which, cudaStream_t st) {
+  int fill(DevModel *M, const LlmqSampling &s, int count, const int *which) {
+    auto &R = M->rows;
     n = static_cast<size_t>(count);
-    std::vector<float> h(5 * n);
+    CK(cudaStreamSynchronize(M->stream));  // a step that failed may have left its copy
+    if (n > R.sample_cap) {
+      cudaFree(R.sample);
+      cudaFreeHost(R.h_sample);
+      R.sample = R.h_sample = nullptr;
+      R.sample_cap = 0;
+      CK(cudaMalloc(&R.sample, 5 * n * sizeof(float)));
+      CK(cudaMallocHost(&R.h_sample, 5 * n * sizeof(float)));
+      R.sample_cap = n;
+    }
     const void *src[5] = {s.temperature, s.top_k, s.top_p, s.min_p, s.u};
     for (int c = 0; c < 5; ++c) {
       has[c] = src[c] != nullptr;
       for (size_t i = 0; i < n && has[c]; ++i)  // 4 bytes each, whatever they mean
-        std::memcpy(&h[c * n + i], static_cast<const char *>(src[c]) + 4 * (which ? (size_t)which[i] : i), 4);
+        std::memcpy(&R.h_sample[c * n + i], static_cast<const char *>(src[c]) + 4 * (which ? (size_t)which[i] : i), 4);
     }
-    CK(cudaMalloc(&dev, 5 * n * sizeof(float)));
-    CK(cudaMemcpyAsync(dev, h.data(), 5 * n * sizeof(float), cudaMemcpyHostToDevice, st));
-    CK(cudaStreamSynchronize(st));  // h ends here
+    CK(cudaMemcpyAsync(R.sample, R.h_sample, 5 * n * sizeof(float), cudaMemcpyHostToDevice, M->stream));
+    dev = R.sample;
     return 1;
   }
   LlmqSampleRows rows(int first) const {
@@ -2044,7 +2056,7 @@ int decode_rows(const QLlamaModel *m, LlamaKV *const *kvs, const int *tokens, in
     ids = tmp.data();
   }
   SampleColumns cols;
-  if (smp && !cols.fill(*smp, B, nullptr, M->stream)) return 0;
+  if (smp && !cols.fill(M, *smp, B, nullptr)) return 0;
   g_launches = 0;
   CK(cudaEventRecord(M->ev0, M->stream));
   for (int off = 0; off < B; off += kRowsPerPass) {

@@ -301,7 +301,7 @@ int paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const 
   if (!paged_reserve(*ctx, M, T, n_active)) return 0;
   std::vector<int> drawn((size_t)n_active);
   SampleColumns cols;
-  if (s && !cols.fill(*s, n_active, active.data(), M->stream)) return 0;
+  if (s && !cols.fill(M, *s, n_active, active.data())) return 0;
   CK(upload_sync(c->added, added, (size_t)c->max_seqs * sizeof(int)));
   CK(upload_sync(c->last, last.data(), last.size() * sizeof(int)));
   // ---- from here on a failure leaves the GPU's tables behind the host's

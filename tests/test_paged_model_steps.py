@@ -9,6 +9,7 @@ import pytest
 
 import llmq
 from helpers import TINY, synth
+from paged_helpers import sample_plain
 from test_paged_model import refused, step
 
 gpu = pytest.mark.gpu
@@ -61,5 +62,73 @@ def test_a_step_the_sampler_would_refuse_is_refused_before_it_runs(lib):
     assert lib.q_llama_paged_free_pages(cache) == 3
     step(lib, m, cache, [1, 20], list(range(21)), 2, want=False)
     assert lib.q_llama_paged_len(cache, 0) == 4 and lib.q_llama_paged_free_pages(cache) == 1
+    lib.q_llama_paged_free(cache)
+    lib.q_llama_model_free(C.byref(m))
+
+
+class Busy:
+    """Half a second of one thread's work on a stream; `running` afterwards: nothing waited for it."""
+
+    def __init__(self, stream):
+        import torch
+        self.stream, self.done = stream, torch.cuda.Event()
+
+    def __enter__(self):
+        import torch
+        torch.cuda.synchronize()
+        with torch.cuda.stream(self.stream):
+            torch.cuda._sleep(1_000_000_000)
+            self.done.record()
+        return self
+
+    def __exit__(self, *_):
+        self.stream.synchronize()
+
+    def running(self):
+        return not self.done.query()
+
+
+@gpu
+def test_sampled_steps_do_not_wait_for_other_streams(lib):
+    import torch
+    m = synth(lib, dict(TINY, n_layers=1), seed=14)
+    kvs = [lib.q_llama_kv_create(C.byref(m)) for _ in range(2)]
+    cache = lib.q_llama_paged_create(C.byref(m), 4, 16, 2, llmq.LLMQ_F32)
+    llmq.check(lib)
+    ids = llmq.int_array([-9, -9])
+    s = llmq.sampling([0.8, 0.8], u=[0.3, 0.6])
+
+    def steps():
+        assert lib.q_llama_decode_batch_sample(C.byref(m), llmq.kv_pointers(kvs), llmq.int_array([5, 6]), 2, C.byref(s),
+                                               ids) == 0
+        step(lib, m, cache, [1, 1], [5, 6], 2, s)
+
+    steps()
+    with Busy(torch.cuda.Stream()) as busy:
+        steps()
+        assert busy.running()
+    for kv in kvs:
+        lib.llama_kv_free(C.byref(kv))
+    lib.q_llama_paged_free(cache)
+    lib.q_llama_model_free(C.byref(m))
+
+
+@gpu
+def test_settings_follow_batches_that_grow_and_shrink(lib):
+    """Batches of other sizes and columns one after another, each by its own settings."""
+    m = synth(lib, dict(TINY, n_layers=1), seed=16, stddev=0.05)
+    g = np.random.default_rng(4)
+    cache = lib.q_llama_paged_create(C.byref(m), 70, 4, 70, llmq.LLMQ_F32)
+    llmq.check(lib)
+    for n in (2, 70, 1, 33):
+        added = [1 if b < n else 0 for b in range(70)]
+        u = g.random(70).astype(np.float32)
+        cols = dict(top_k=g.integers(1, 50, 70)) if n % 2 else dict(temperature=g.choice([0.7, 1.3], 70), min_p=[0.01] * 70)
+        ids, rows = step(lib, m, cache, added, g.integers(0, m.vocab, n).tolist(), 70, llmq.sampling(u=u, **cols))
+        for b in range(n):
+            want, _, margin = sample_plain(rows[b], float(np.float32(cols.get("temperature", [1.0] * 70)[b])),
+                                           int(cols.get("top_k", [0] * 70)[b]), 1.0,
+                                           float(np.float32(cols.get("min_p", [0.0] * 70)[b])), float(u[b]))
+            assert margin < m.vocab * 2.0 ** -44 or ids[b] == want
     lib.q_llama_paged_free(cache)
     lib.q_llama_model_free(C.byref(m))
