@@ -14,6 +14,7 @@ struct LlmqPagedCache {
   char *k = nullptr, *v = nullptr;  // [layer][page][position][head][head_dim]
   int *table = nullptr, *lens = nullptr, *first = nullptr, *added = nullptr, *free_pages = nullptr, *head = nullptr;
   int *status = nullptr, *last = nullptr;  // last: the rows the lm-head takes
+  int *h_step = nullptr;                   // pinned: added [max_seqs], then last [max_seqs]
   float *x = nullptr;                      // [max_seqs][d_model]: their residual stream
   void *work = nullptr;
   size_t work_bytes = 0;
@@ -36,6 +37,7 @@ void release_paged(LlmqPagedCache *c) {
   void *p[] = {c->k,      c->v,    c->table, c->lens,      c->first, c->added, c->free_pages, c->head, c->status,
                c->last,   c->x,    c->work,  c->slots,     c->positions, c->seqs, c->spans};
   for (void *q : p) cudaFree(q);
+  cudaFreeHost(c->h_step);
   delete c;
 }
 
@@ -156,6 +158,7 @@ LlmqPagedCache *paged_create(const QLlamaModel *m, int n_pages, int page_size, i
     CK(cudaMalloc(&c->v, pool));
     CK(cudaMalloc(&c->work, c->work_bytes));
     CK(cudaMalloc(&c->table, (size_t)max_seqs * c->max_pages * sizeof(int)));
+    CK(cudaMallocHost(&c->h_step, 2 * (size_t)max_seqs * sizeof(int)));
     CK(cudaMalloc(&c->x, (size_t)max_seqs * cfg.d_model * sizeof(float)));
     if (!dev_zeros(&c->lens, max_seqs) || !dev_zeros(&c->first, (size_t)max_seqs + 1) || !dev_zeros(&c->added, max_seqs) ||
         !dev_zeros(&c->head, 1) || !dev_zeros(&c->status, 1) || !dev_zeros(&c->last, max_seqs) ||
@@ -179,6 +182,7 @@ LlmqPagedCache *paged_create(const QLlamaModel *m, int n_pages, int page_size, i
 }
 
 int paged_reset(LlmqPagedCache *c, int seq) {
+  const cudaStream_t st = c->model->stream;
   std::vector<int> &own = c->pages[(size_t)seq];
   std::vector<int> next;
   if (!own.empty()) {
@@ -187,13 +191,16 @@ int paged_reset(LlmqPagedCache *c, int seq) {
   }
   c->broken = true;  // a failure from here on leaves the GPU's lists behind the host's
   if (!own.empty()) {
-    CK(upload_sync(c->free_pages, next.data(), next.size() * sizeof(int)));
-    CK(zero_sync(c->head, sizeof(int)));
+    CK(cudaMemcpyAsync(c->free_pages, next.data(), next.size() * sizeof(int), cudaMemcpyHostToDevice, st));
+    CK(cudaMemsetAsync(c->head, 0, sizeof(int), st));
+  }
+  CK(cudaMemsetAsync(c->lens + seq, 0, sizeof(int), st));
+  CK(cudaStreamSynchronize(st));  // `next` has been read
+  if (!own.empty()) {
     c->free_list.swap(next);
     c->head_h = 0;
     own.clear();
   }
-  CK(zero_sync(c->lens + seq, sizeof(int)));
   c->len[(size_t)seq] = 0;
   c->broken = false;
   return 1;
@@ -302,10 +309,12 @@ int paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const 
   std::vector<int> drawn((size_t)n_active);
   SampleColumns cols;
   if (s && !cols.fill(M, *s, n_active, active.data())) return 0;
-  CK(upload_sync(c->added, added, (size_t)c->max_seqs * sizeof(int)));
-  CK(upload_sync(c->last, last.data(), last.size() * sizeof(int)));
   // ---- from here on a failure leaves the GPU's tables behind the host's
   c->broken = true;
+  std::copy(added, added + c->max_seqs, c->h_step);
+  std::copy(last.begin(), last.end(), c->h_step + c->max_seqs);
+  CK(cudaMemcpyAsync(c->added, c->h_step, (size_t)c->max_seqs * sizeof(int), cudaMemcpyHostToDevice, M->stream));
+  CK(cudaMemcpyAsync(c->last, c->h_step + c->max_seqs, last.size() * sizeof(int), cudaMemcpyHostToDevice, M->stream));
   g_launches = 0;
   CK(cudaEventRecord(M->ev0, M->stream));
   LlmqPagedPlan plan{};

@@ -132,3 +132,19 @@ def test_settings_follow_batches_that_grow_and_shrink(lib):
             assert margin < m.vocab * 2.0 ** -44 or ids[b] == want
     lib.q_llama_paged_free(cache)
     lib.q_llama_model_free(C.byref(m))
+
+
+@gpu
+def test_steps_and_resets_do_not_wait_for_the_default_stream(lib):
+    import torch
+    m = synth(lib, dict(TINY, n_layers=1), seed=15)
+    cache = lib.q_llama_paged_create(C.byref(m), 4, 16, 2, llmq.LLMQ_F32)
+    llmq.check(lib)
+    first, want = step(lib, m, cache, [5, 1], [1, 2, 3, 4, 5, 9], 2)
+    with Busy(torch.cuda.default_stream()) as busy:
+        assert lib.q_llama_paged_reset(cache, 0) == 0 and lib.q_llama_paged_reset(cache, 1) == 0
+        ids, rows = step(lib, m, cache, [5, 1], [1, 2, 3, 4, 5, 9], 2)
+        assert busy.running()
+    assert ids == first and np.array_equal(rows.view(np.uint32), want.view(np.uint32))
+    lib.q_llama_paged_free(cache)
+    lib.q_llama_model_free(C.byref(m))
