@@ -285,10 +285,11 @@ int paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const 
     }
     rows[r] = RowDesc{nullptr, nullptr, 0, 0, tokens[r], 0};
   }
-  std::vector<std::vector<int>> pages_after = c->pages;
-  int head_after = c->head_h;
-  for (int b = 0; b < c->max_seqs; ++b)
-    for (int i = 0; i < need[b]; ++i) pages_after[b].push_back(c->free_list[head_after++]);
+  for (int b : active) {  // room for the pages it takes, so that noting them cannot fail
+    std::vector<int> &own = c->pages[b];
+    const size_t n = own.size() + need[b];
+    if (n > own.capacity()) own.reserve(std::max(n, 2 * own.capacity()));
+  }
   if (T > c->cap) {
     void *old[] = {c->slots, c->positions, c->seqs, c->spans};
     for (void *p : old) cudaFree(p);
@@ -370,11 +371,11 @@ int paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const 
     return 0;
   }
   c->broken = false;
-  c->pages.swap(pages_after);
-  c->head_h = head_after;
   for (int i = 0; i < n_active; ++i) {
-    c->len[active[i]] += added[active[i]];
-    ids[active[i]] = drawn[i];
+    const int b = active[i];
+    for (int k = 0; k < need[b]; ++k) c->pages[b].push_back(c->free_list[c->head_h++]);
+    c->len[b] += added[b];
+    ids[b] = drawn[i];
   }
   return 1;
 }
