@@ -301,8 +301,9 @@ void q_llama_prefill(const QLlamaModel *m, LlamaKV *kv, const int *ids, int n, T
  * on error. */
 int q_llama_prefill_argmax(const QLlamaModel *m, LlamaKV *kv, const int *ids, int n, Tensor *logits);
 
-/* Kernels launched by the last q_llama_decode_batch[_argmax] or
- * q_llama_prefill[_argmax] call (diagnostic; no reference counterpart). */
+/* Kernels launched by the last q_llama_decode_batch[_argmax|_sample],
+ * q_llama_paged_step or q_llama_prefill[_argmax] call (diagnostic; no reference
+ * counterpart). */
 long long llmq_last_launches(void);
 
 /* ---- Tensor parallelism (the `q_llama_tp_init` extension; the reference is

@@ -155,6 +155,7 @@ void free_matf(MatF &m) {
 int g_smem_optin = 0;
 long long g_launches = 0;       // kernels launched by the running multi-row call
 long long g_last_launches = 0;  // ... by the last completed one
+thread_local long long t_serve_launches = 0;  // by this thread's serving operators, which take no lock
 
 // ------------------------------------------------------ tensor parallelism
 // One process per GPU; the ranks of a tensor-parallel group share an NCCL
@@ -2058,6 +2059,7 @@ int decode_rows(const QLlamaModel *m, LlamaKV *const *kvs, const int *tokens, in
   SampleColumns cols;
   if (smp && !cols.fill(M, *smp, B, nullptr)) return 0;
   g_launches = 0;
+  const long long served = t_serve_launches;
   CK(cudaEventRecord(M->ev0, M->stream));
   for (int off = 0; off < B; off += kRowsPerPass) {
     const int n = std::min(kRowsPerPass, B - off);
@@ -2074,7 +2076,7 @@ int decode_rows(const QLlamaModel *m, LlamaKV *const *kvs, const int *tokens, in
   CK(cudaEventRecord(M->ev1, M->stream));
   CK(cudaEventSynchronize(M->ev1));
   cudaEventElapsedTime(&g_last_ms, M->ev0, M->ev1);
-  g_last_launches = g_launches;
+  g_last_launches = g_launches + t_serve_launches - served;
   return 1;
 }
 
@@ -2494,6 +2496,8 @@ int llmqd_tp_world(void) { return g_tp.world; }
 
 // ---- diagnostics exported for tests and the benchmark (declared in llmq_cuda.h)
 LLMQ_API long long llmq_last_launches(void) { return g_last_launches; }
+
+void llmqd_count_launch(void) { ++t_serve_launches; }
 
 LLMQ_API int llmq_expf_device(const float *x, float *y, long long n) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);

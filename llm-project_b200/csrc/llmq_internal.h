@@ -81,6 +81,8 @@ LLMQ_HIDDEN int llmqd_decode_f32(const LlamaModel *m, const LlamaKV *kv, int tok
 /* n device-chained steps (greedy, or drawn when smp is set). */
 LLMQ_HIDDEN int llmqd_generate_f32(const LlamaModel *m, const LlamaKV *kv, int token, int n, int *ids,
                                    LlmqSample *smp);
+/* A serving operator has launched a kernel on this thread (llmq_last_launches). */
+LLMQ_HIDDEN void llmqd_count_launch(void);
 /* Size of this process's tensor-parallel group (1 if none). */
 LLMQ_HIDDEN int llmqd_tp_world(void);
 

@@ -317,6 +317,7 @@ int paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const 
   CK(cudaMemcpyAsync(c->added, c->h_step, (size_t)c->max_seqs * sizeof(int), cudaMemcpyHostToDevice, M->stream));
   CK(cudaMemcpyAsync(c->last, c->h_step + c->max_seqs, last.size() * sizeof(int), cudaMemcpyHostToDevice, M->stream));
   g_launches = 0;
+  const long long served = t_serve_launches;
   CK(cudaEventRecord(M->ev0, M->stream));
   LlmqPagedPlan plan{};
   plan.n_seqs = c->max_seqs;
@@ -365,7 +366,7 @@ int paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const 
   CK(cudaEventRecord(M->ev1, M->stream));
   CK(cudaStreamSynchronize(M->stream));
   cudaEventElapsedTime(&g_last_ms, M->ev0, M->ev1);
-  g_last_launches = g_launches;
+  g_last_launches = g_launches + t_serve_launches - served;
   if (flags) {
     llmq_set_error(LLMQ_ERR_CUDA, "%s: the paged cache reported flags 0x%x", fn, flags);
     return 0;

@@ -1529,6 +1529,7 @@ cudaError_t launch_clusters(void (*kern)(RowArgs), const RowArgs &p, int ctas, i
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
+  llmqd_count_launch();
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 

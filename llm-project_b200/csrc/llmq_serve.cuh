@@ -77,6 +77,7 @@ inline cudaError_t serve_launch(void (*kern)(KArgs...), dim3 grid, dim3 block, s
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
+  llmqd_count_launch();
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 

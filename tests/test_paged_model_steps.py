@@ -148,3 +148,28 @@ def test_steps_and_resets_do_not_wait_for_the_default_stream(lib):
     assert ids == first and np.array_equal(rows.view(np.uint32), want.view(np.uint32))
     lib.q_llama_paged_free(cache)
     lib.q_llama_model_free(C.byref(m))
+
+
+@gpu
+def test_launches_of_sampled_and_paged_steps(lib):
+    """The sampler is one more kernel than the greedy step; over pages a layer has the writer,
+    attention and its join in place of the writer, scores and values, and the step a plan and
+    a copy of its last rows besides."""
+    m = synth(lib, TINY, seed=17)
+    kvs = [lib.q_llama_kv_create(C.byref(m)) for _ in range(2)]
+    cache = lib.q_llama_paged_create(C.byref(m), 32, 16, 2, llmq.LLMQ_F32)
+    llmq.check(lib)
+    toks, ids = llmq.int_array([5, 6]), llmq.int_array([-9, -9])
+    s = llmq.sampling([0.8, 0.8], u=[0.3, 0.6])
+    assert lib.q_llama_decode_batch_argmax(C.byref(m), llmq.kv_pointers(kvs), toks, 2, ids) == 0
+    greedy = lib.llmq_last_launches()
+    assert lib.q_llama_decode_batch_sample(C.byref(m), llmq.kv_pointers(kvs), toks, 2, C.byref(s), ids) == 0
+    assert lib.llmq_last_launches() == greedy + 1
+    step(lib, m, cache, [1, 1], [5, 6], 2)
+    assert lib.llmq_last_launches() == greedy + 2
+    step(lib, m, cache, [1, 1], [5, 6], 2, s)
+    assert lib.llmq_last_launches() == greedy + 3
+    for kv in kvs:
+        lib.llama_kv_free(C.byref(kv))
+    lib.q_llama_paged_free(cache)
+    lib.q_llama_model_free(C.byref(m))
