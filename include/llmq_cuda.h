@@ -627,11 +627,12 @@ int llmq_paged_append(const LlmqPagedKV *kv, const LlmqPagedAppend *a, void *str
  * formed in f32 and rounded once; over a 16-bit pool the weights multiply the
  * values as sums of 16-bit terms (16 bits of a weight for bf16 rows, 22 for f16
  * pools, 24 for f32 rows over bf16).  The result depends on the batch only in
- * the order of its sums.  A row without positions gives zeros and lse -infinity.
- * Positions on a page outside the pool are left out.  What the pool holds past
- * a row's length is never read into a result.  out may not overlap q.  scale 0
- * stands for 1 / sqrt(head_dim).  The workspace need not be initialised; calls that may
- * overlap need one each. */
+ * the order of its sums.  A row without positions gives zeros and lse -infinity;
+ * a head with a NaN or +infinite score (of NaN or infinities in its q or used
+ * keys) gives NaN for both.  Positions on a page outside the pool are left out.
+ * What the pool holds past a row's length is never read into a result.  out may
+ * not overlap q.  scale 0 stands for 1 / sqrt(head_dim).  The workspace need not
+ * be initialised; calls that may overlap need one each. */
 typedef struct {
   int n_rows, n_heads;
   int dtype;     /* of q and out */

@@ -111,6 +111,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return *reinterpret_cast<float2 *>(&r);
 }
 
+// Of a reference m and the sum of 2^(s - m): 1 / sum and ln of what it stands for.  A sum of 0
+// is a head without positions; a NaN (of a NaN or +infinite score) goes on into both.
+__device__ __forceinline__ float share_of(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+__device__ __forceinline__ float lse_of(float m, float sum) {
+  return sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+}
+
 // What one row attends: positions [n0, n) in tiles [t0, t0 + tiles).
 struct RowSpan {
   long long seq;
@@ -824,13 +831,13 @@ __global__ void __launch_bounds__(kAttendThreads, AttendShape<Core, HDP>::kPerSm
           sum += h < nh ? of(w).l(h) * f : 0.0f;
           s_factor[w][h] = f;
         }
-        s_inv[h] = out_now ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
+        s_inv[h] = out_now ? share_of(sum) : 1.0f;
         if (h < nh) {
           if (!out_now) {
             part[h] = mx;
             part[kHeadBlock + h] = sum;
           } else if (a.lse) {
-            a.lse[(size_t)at.row * a.n_heads + h0 + h] = sum > 0.0f ? (mx + log2f(sum)) * 0.693147180559945309f : -INFINITY;
+            a.lse[(size_t)at.row * a.n_heads + h0 + h] = lse_of(mx, sum);
           }
         }
       }
@@ -966,7 +973,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendArgs p
       v.z += x.z;
       v.w += x.w;
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float inv = share_of(sum);
     T *o = static_cast<T *>(a.out) + at.row * a.out_stride + (size_t)head * hd + d;
     o[0] = from_f32<T>(v.x * inv);
     o[1] = from_f32<T>(v.y * inv);
@@ -974,7 +981,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const AttendArgs p
     o[3] = from_f32<T>(v.w * inv);
   }
   if (tid == 0 && a.lse)
-    a.lse[(size_t)at.row * a.n_heads + head] = sum > 0.0f ? (mx + log2f(sum)) * 0.693147180559945309f : -INFINITY;
+    a.lse[(size_t)at.row * a.n_heads + head] = lse_of(mx, sum);
 }
 
 }  // namespace llmq
