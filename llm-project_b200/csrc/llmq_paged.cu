@@ -322,6 +322,19 @@ extern "C" LLMQ_API int llmq_paged_plan(const LlmqPagedPlan *a, void *stream) {
   c.require(a->table_stride >= a->max_pages, "table_stride is below max_pages");
   c.require(a->n_seqs == 0 || (a->cached && a->added && a->table && a->lens), "null pointer");
   c.require(a->first && (a->max_rows == 0 || a->slots) && (a->n_free == 0 || a->free_pages), "null pointer");
+  c.elements(a->cached, "cached");
+  c.elements(a->added, "added");
+  c.elements(a->free_pages, "free_pages");
+  c.elements(a->free_head, "free_head");
+  c.elements(a->table, "table");
+  c.elements(a->lens, "lens");
+  c.elements(a->first, "first");
+  c.elements(a->slots, "slots");
+  c.elements(a->positions, "positions");
+  c.elements(a->seqs, "seqs");
+  c.elements(a->spans, "spans");
+  c.elements(a->next_head, "next_head");
+  c.elements(a->status, "status");
   c.on_device();
   c.memory(a->cached, "cached");
   c.memory(a->added, "added");
@@ -447,6 +460,11 @@ extern "C" LLMQ_API int llmq_paged_append(const LlmqPagedKV *kv, const LlmqPaged
   const size_t e = c.rc == LLMQ_OK ? serve_bytes(a->dtype) : 1;
   c.require(aligned_to(a->q, e) && aligned_to(a->k, e) && aligned_to(a->v, e) && aligned_to(a->q_out, e),
             "a row does not start on an element");
+  c.elements(a->slots, "slots");
+  c.elements(a->positions, "positions");
+  c.elements(a->rope_cos, "rope_cos");
+  c.elements(a->rope_sin, "rope_sin");
+  c.elements(a->status, "status");
   c.on_device();
   c.memory(kv->k, "the pool");
   c.memory(kv->v, "the pool");
@@ -496,6 +514,11 @@ extern "C" LLMQ_API int llmq_paged_attention(const LlmqPagedKV *kv, const LlmqPa
   c.require(a->q_stride >= qd && a->out_stride >= qd, "a row stride is shorter than its row");
   const size_t e = c.rc == LLMQ_OK ? serve_bytes(a->dtype) : 1;
   c.require(aligned_to(a->q, e) && aligned_to(a->out, e), "a row does not start on an element");
+  c.elements(a->lse, "lse");
+  c.elements(a->table, "table");
+  c.elements(a->seqs, "seqs");
+  c.elements(a->lens, "lens");
+  c.elements(a->status, "status");
   if (c.rc != LLMQ_OK) return c.rc;
   const size_t need = llmq_paged_attention_workspace(a->n_rows, a->n_heads, kv->n_kv, kv->head_dim);
   c.require(a->workspace && a->workspace_bytes >= need && aligned16(a->workspace),

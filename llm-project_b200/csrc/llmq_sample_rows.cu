@@ -1576,6 +1576,13 @@ extern "C" LLMQ_API int llmq_sample_rows(const LlmqSampleRows *a, void *stream) 
   c.require(a->logits && a->u && a->ids, "null pointer");
   c.require(a->stride >= a->vocab, "a row stride is shorter than its row");
   c.require(aligned_to(a->logits, serve_bytes(a->dtype)), "the logits do not start on an element");
+  c.elements(a->temperature, "temperature");
+  c.elements(a->top_k, "top_k");
+  c.elements(a->top_p, "top_p");
+  c.elements(a->min_p, "min_p");
+  c.elements(a->u, "u");
+  c.elements(a->ids, "ids");
+  c.elements(a->logprobs, "logprobs");
   c.on_device();
   c.memory(a->logits, "logits");
   c.memory(a->temperature, "temperature");

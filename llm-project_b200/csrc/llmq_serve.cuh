@@ -25,6 +25,13 @@ struct ServeCheck {
     rc = LLMQ_ERR_ARG;
     llmq_set_error(rc, "%s: %s", fn, what);
   }
+  // Arrays of T start on one: the kernels load and store whole elements.
+  template <typename T>
+  void elements(const T *p, const char *what) {
+    if (rc != LLMQ_OK || reinterpret_cast<uintptr_t>(p) % sizeof(T) == 0) return;
+    rc = LLMQ_ERR_ARG;
+    llmq_set_error(rc, "%s: %s does not start on an element", fn, what);
+  }
   void on_device() {
     if (rc != LLMQ_OK) return;
     int major = 0;
