@@ -529,7 +529,8 @@ int qmatmul_device_noalloc(const float *A, int M, int K, const signed char *Wq, 
  * or a workspace.  Pointers marked "or NULL" are optional.  Sizes, strides and
  * null pointers are checked on the host, and so is that every array starts on
  * one of its elements and is memory of the current GPU; a call that fails one of these checks returns
- * LLMQ_ERR_ARG and enqueues nothing.  Values that only the GPU sees (lengths,
+ * LLMQ_ERR_ARG and enqueues nothing.  n_rows and n_seqs stay below 2^31 - 4096,
+ * a row's elements below 2^31.  Values that only the GPU sees (lengths,
  * page ids, slots, positions) are checked there: an entry out of range is left
  * out and its flag is OR'ed into *status (a device int the caller has zeroed, or
  * NULL).  Unused descriptor fields must be zero.  Strides count elements.

@@ -317,6 +317,7 @@ extern "C" LLMQ_API int llmq_paged_plan(const LlmqPagedPlan *a, void *stream) {
   c.require(a != nullptr, "null descriptor");
   if (c.rc != LLMQ_OK) return c.rc;
   c.require(a->n_seqs >= 0 && a->max_rows >= 0 && a->n_free >= 0, "negative size");
+  c.require(a->n_seqs <= kServeMaxRows, "n_seqs is above 2^31 - 4097");
   c.require(a->page_size > 0 && a->max_pages > 0 && (long long)a->page_size * a->max_pages <= INT_MAX,
             "page_size and max_pages must be above 0 and their product below 2^31");
   c.require(a->table_stride >= a->max_pages, "table_stride is below max_pages");
@@ -447,6 +448,8 @@ extern "C" LLMQ_API int llmq_paged_append(const LlmqPagedKV *kv, const LlmqPaged
   if (c.rc != LLMQ_OK) return c.rc;
   check_types(c, a->dtype, kv->dtype);
   c.require(a->n_rows >= 0 && a->n_heads >= 0 && a->rope_len >= 0, "negative size");
+  c.require(a->n_rows <= kServeMaxRows, "n_rows is above 2^31 - 4097");
+  c.require((long long)a->n_heads * kv->head_dim <= INT_MAX, "a row has 2^31 elements or more");
   if (c.rc != LLMQ_OK || a->n_rows == 0) return c.rc;
   c.require(a->k && a->v && a->slots, "null pointer");
   c.require((a->n_heads > 0) == (a->q != nullptr) && (a->q != nullptr) == (a->q_out != nullptr),
@@ -502,7 +505,9 @@ extern "C" LLMQ_API int llmq_paged_attention(const LlmqPagedKV *kv, const LlmqPa
   if (c.rc != LLMQ_OK) return c.rc;
   check_types(c, a->dtype, kv->dtype);
   c.require(a->n_rows >= 0 && a->n_seqs >= 0 && a->max_pages >= 0 && a->window >= 0, "negative size");
+  c.require(a->n_rows <= kServeMaxRows, "n_rows is above 2^31 - 4097");
   c.require(a->n_heads > 0 && a->n_heads % kv->n_kv == 0, "n_heads must be a multiple of n_kv");
+  c.require((long long)a->n_heads * kv->head_dim <= INT_MAX, "a row has 2^31 elements or more");
   // (a tile may reach past the last position: room for it below 2^31)
   c.require((long long)a->max_pages * kv->page_size <= INT_MAX - 4096, "max_pages * page_size must stay below 2^31 - 4096");
   c.require(a->table_stride >= a->max_pages, "table_stride is below max_pages");

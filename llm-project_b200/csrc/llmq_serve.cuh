@@ -64,6 +64,10 @@ struct ServeCheck {
   }
 };
 
+// Rows or requests of a call: kernels and launch loops step over them in ints, by blocks of
+// at most 4096.
+constexpr int kServeMaxRows = 0x7fffffff - 4096;
+
 inline bool serve_dtype(int t) { return t == LLMQ_F32 || t == LLMQ_F16 || t == LLMQ_BF16; }
 inline size_t serve_bytes(int t) { return t == LLMQ_F32 ? 4 : 2; }
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
