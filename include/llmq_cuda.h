@@ -668,11 +668,14 @@ size_t llmq_paged_attention_workspace(int n_rows, int n_heads, int n_kv, int hea
  * sum of w reaches top_p of the whole row's (off: outside (0, 1)).  The token
  * drawn is the first one, in that order, at which the sum of w reaches u times
  * the kept sum; u is clamped to [0, 1] (NaN: 0).  A temperature that is not above
- * 0 (NaN too) takes the first largest logit.  Sums are exact to 2^-42 of the
- * largest w or better (64-bit integers, the same in any order), so a row's
- * token does not depend on the batch it is in.  A NaN or -infinite logit is
- * never drawn; a row of nothing else gives id -1 and logprob -infinity; among
- * +infinite logits the weights are equal.
+ * 0 (NaN too) takes the first largest logit.  Each w is rounded to a multiple of
+ * 2^-S, S = min(50, 62 - ceil(log2 vocab)): one below 2^-(S+1) counts as nothing.
+ * Sums of those are exact, the same in any order, so a row's token does not depend
+ * on the batch it is in; a sum is within vocab * 2^-S of the real one (half of it
+ * from rounding, 2^-29 at 128256 tokens; the rest covers the exponential), and
+ * only a border nearer than that to a choice may fall to either neighbour.  A NaN
+ * or -infinite logit is never drawn; a row of nothing else gives id -1 and logprob
+ * -infinity; among +infinite logits the weights are equal.
  * logprobs[r] is the log of the drawn token's share of the kept sum (0 for the
  * greedy choice). */
 typedef struct {
@@ -710,9 +713,9 @@ int q_llama_decode_batch_sample(const QLlamaModel *m, LlamaKV **kvs, const int *
 /* A paged cache of up to max_seqs sequences of a model: n_pages pages of
  * page_size positions (of every layer), shared out as the sequences grow, in
  * place of one max_seq cache a sequence (n_pages * page_size < 2^31 - 4096).
- * dtype is the pages' type; sequences start empty.  head_dim must be a multiple of 8, at most 256.  Not under tensor
- * parallelism.  NULL on error.  The cache belongs to the model: freeing the model
- * frees it (the handle is then invalid). */
+ * dtype is the pages' type; sequences start empty.  head_dim must be a multiple
+ * of 8, at most 256.  Not under tensor parallelism.  NULL on error.  The cache
+ * belongs to the model: freeing the model frees it (the handle is then invalid). */
 typedef struct LlmqPagedCache LlmqPagedCache;
 LlmqPagedCache *q_llama_paged_create(const QLlamaModel *m, int n_pages, int page_size, int max_seqs, int dtype);
 void q_llama_paged_free(LlmqPagedCache *c);
@@ -732,11 +735,11 @@ int q_llama_paged_reset(LlmqPagedCache *c, int seq);
  * sequences that took tokens, in their order.  Attention runs as documented at
  * llmq_paged_attention: unlike q_llama_decode_batch it does not keep the
  * reference's order of additions, so logits are near that path's, not equal bit
- * for bit.  A row reads its sequence's keys and values on its own: made for decode
- * steps and short prompts; q_llama_prefill is the one that shares them among a
- * prompt's rows.  An error leaves the sequences as they were; after one of the GPU
- * in the middle of a step the cache answers LLMQ_ERR_STATE until it is freed.
- * Returns 0 or an error code. */
+ * for bit.  Each row of a prompt reads its sequence's keys and values on its own,
+ * so a prompt's reads grow with the square of its length.  An error leaves the
+ * sequences as they were (LLMQ_ERR_OOM: pages, or memory for so many rows, ran
+ * out); after one of the GPU in the middle of a step the cache answers
+ * LLMQ_ERR_STATE until it is freed.  Returns 0 or an error code. */
 int q_llama_paged_step(const QLlamaModel *m, LlmqPagedCache *c, const int *added, const int *tokens,
                        const LlmqSampling *s, int *ids, Tensor *logits);
 

@@ -208,8 +208,9 @@ constexpr int kAppendThreads = 256;
 constexpr int kHeadLanes = 8;
 
 // What bounds it: the rows' bytes, read once and written once.  16384 bf16 rows of 32 query
-// heads and 8 KV heads of 128 (404 MB) take 70.7 us, 5.7 TB/s of the 6.46 a plain copy
-// moves; 64 rows 3.3 us and one 1.9 us, the latency of a launch and two dependent loads.
+// heads and 8 KV heads of 128 (404 MB) take 70.9 us, 5.7 TB/s of the 6.46 a plain copy
+// moves; 64 rows 4.1 us (3.3 from L2) and one 1.9 us, the latency of a launch and two
+// dependent loads.
 //
 // A thread owns VN adjacent pairs (d, d + head_dim / 2) of every `lanes`th head of a row:
 // the pairs' angles are read once and serve its heads.  The next head's loads are on

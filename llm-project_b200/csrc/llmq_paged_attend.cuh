@@ -20,14 +20,19 @@
 // a page outside the pool are filled with zeros and masked, so what memory
 // holds there (NaN too) is never used.
 //
-// Measured, both kernels (a plain copy moves 6.46 TB/s on the same GPU), 32 query heads
-// (the long row: 64) on 8 KV heads of 128:
-//   64 f32 rows of about 2100 positions      186 us, 5.98 TB/s (203 us under minutes of load)
-//   61 bf16 rows of up to 8191 positions     189 us, 5.94 TB/s
-//   one f16 row of 131072 positions           97 us, 5.52 TB/s: 6.95 TB/s in the long run
-//     and some 17 us that do not depend on the length (launch, prefix sums, the first
+// Measured, both kernels in a captured graph (a plain copy moves 6.46 TB/s on the same GPU),
+// 32 query heads (the long row: 64) on 8 KV heads of 128; in brackets calls in turn under
+// seconds of load:
+//   64 f32 rows of about 2100 positions      185 us, 5.99 TB/s (209 us, 5.32)
+//   61 bf16 rows of up to 8191 positions     189 us, 5.94 TB/s (199 us, 5.63)
+//   64 f32 rows over bf16, 2112 positions    100 us, 5.53 TB/s
+//   one f16 row of 131072 positions           98 us, 5.45 TB/s (101 us): 6.95 TB/s in the long
+//     run and some 17 us that do not depend on the length (launch, prefix sums, the first
 //     loads' latency, the join)
+//   8 bf16 rows of 512, 1024, 2048 positions  15, 18, 22 us, for 2.6, 5.2, 10.4 at the copy's rate
 //   one row of a few hundred positions         7 us, the same chain without the bytes
+//   16 bf16 rows of 4096, 16 query heads a KV head: 51 us, two readings of the 135 MB (20.8 for
+//     one at the copy's rate)
 // Counters at 16 rows of 2100: the cache read once (280 MB of DRAM reads for 278 MB), 42%
 // (f32) and 33% (bf16) of the issue slots, 2 CTAs of 4 warps an SM (180 and 207
 // registers): the ring, not the warps, keeps the memory busy.

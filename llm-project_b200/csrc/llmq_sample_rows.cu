@@ -11,7 +11,9 @@
 // by its sum alone, and the draw is the first token at which the sum reaches u
 // times the kept one.  No cut needs a sorted row: only the tokens around it.
 //
-// A cluster of CTAs holds a row in shared memory, read from DRAM once:
+// A cluster of CTAs shares a row, which is read from DRAM once: each CTA keeps its slice in
+// shared memory if that has room (64 KB: 8 CTAs for 128256 f32 logits, 4 for f16), else
+// later passes read it from L2.
 //  1. The largest and least logit, and for a top_k up to 96 the largest of each of
 //     128 groups of tokens: the k-th largest of those is a bound that at least k
 //     tokens reach and few more do (k = 40: about 48 of a smooth row's).  A min_p
@@ -29,10 +31,12 @@
 // What bounds it is not DRAM but instructions and latency: a weight costs some 30
 // instructions (doubles, for the exact sum), the histogram two shared atomics a token.
 // Measured: 64 f32 rows of 128256 with mixed settings (32.8 MB, 5.1 us at a plain copy's
-// rate) 52.4 us, the rows without a bound last longest; the same rows with a top_k of 50,
-// no exponential but the list's, 24 us; one row of 32000, top_k 40 and top_p, 10.6 us, a
-// chain of cluster barriers.  Counters for the mixed rows: 33.0 MB read, 40% of the issue
-// slots, two further turns of a shared atomic for equal banks.
+// rate) 56 to 59 us, the time of their rows without a bound, which share 4 CTAs like all
+// others (64 of those alone: 58; 256: 161; f16: 57 and 151); the same rows with a top_k of 50,
+// no exponential but the list's, 24 us, and with a top_k of 40 and a top_p, which asks for the
+// whole sum, 37.5; one row of 32000 so 10.5 us, a chain of cluster barriers.  Counters for
+// the mixed rows: 33.0 MB read, 40% of the issue slots, two further turns of a shared
+// atomic for equal banks.
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -567,9 +571,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(const RowArgs p) {
   // stride up to 32 stay within its 64 items: only larger strides need the other warps,
   // and a list of up to 64 items one warp alone.
   // Up to kCounted items are put in place by counting what precedes each, several
-  // threads an item; the sorted items are then in `gathered`.  (64 rows of top_k 50, whose
-  // lists hold some 60: 37.7 us, 40.3 sorted; nucleus rows, of a few hundred: 59.5 us
-  // counted up to 512, 57.8 up to 256.)
+  // threads an item; the sorted items are then in `gathered`.  (64 f32 rows of 128256 with a
+  // top_k of 50, whose lists hold some 60: 24.2 us, 26.7 sorted; nucleus rows, of a few
+  // hundred: 60.7 us counted up to 512, 58.0 up to 256.)
   constexpr int kCounted = 256;
   static_assert(kCounted <= kThreads, "a thread an item");
   u64 *items = list;
@@ -1537,8 +1541,8 @@ cudaError_t launch_values(const LlmqSampleRows &a, int sms, cudaStream_t st) {
   RowArgs p{};
   p.a = a;
   p.scale = scale_bits(a.vocab);
-  // CTAs a row until every SM has one: 128 rows 39 us in clusters of 2, 48 of 4; 256 rows
-  // 66 us alone, 73 in clusters of 2
+  // CTAs a row until every SM has one (rows of 128256): 128 rows 38 us in clusters of 2, 44
+  // alone, 45 of 4; 256 rows 63 us alone, 68 in clusters of 2
   int ctas = 1;
   while (ctas < kMaxCluster && (long long)a.n_rows * ctas < sms && a.vocab / ctas > 4 * kValueThreads) ctas *= 2;
   p.slice = ((a.vocab + ctas - 1) / ctas + 15) / 16 * 16;
@@ -1553,7 +1557,8 @@ cudaError_t launch(const LlmqSampleRows &a, int sms, cudaStream_t st) {
   p.a = a;
   p.scale = scale_bits(a.vocab);
   // CTAs a row: as many as let all rows be on the GPU at once, two CTAs an SM.  (64 rows of
-  // 128256 f32 logits, top-k 50: 24 us in clusters of 4, 34 us of 8, which take two turns.)
+  // 128256 f32 logits, top-k 50: 24 us in clusters of 4, 35 us of 8, which take two turns,
+  // 31 of 2.)
   int ctas = 1;
   auto slice_of = [&](int c) { return ((a.vocab + c - 1) / c + 15) / 16 * 16; };
   while (ctas < kMaxCluster && 2LL * a.n_rows * ctas <= 2 * sms && slice_of(ctas) > 2 * kThreads) ctas *= 2;
